@@ -1,0 +1,368 @@
+// Attention of a tree of drafted tokens over the paged cache: node i of a sequence sees the cached keys and the nodes that its
+// mask names (its ancestors and itself),
+//   o_i = sum_j a_ij v_j / (sum_j a_ij + exp(sink)),   a_ij = exp(f(scale q_i . k_j)),   f(x) = x or c tanh(x / c),
+// where with a window w only keys within w positions before the node's own position count (a node's position is its depth
+// behind the cached tokens, not its index in the cache). A row that sees no key is 0. Keys and values of masked places never
+// reach a result, whatever they hold.
+//
+// This file: the general kernel (float32 and bfloat16, any key and value size up to 512, any head ratio, both tile
+// layouts; all arithmetic float32 with expf and tanhf), and the kernel that joins the segments of both this one and
+// the tensor-core kernel of attn_tree_tc.cu.
+//
+// General kernel: a block has 32 rows (node, query head) of one kv head and a segment of the keys, and takes a page (64 keys)
+// at a time through shared memory in float32, keys and then values in the same place: scores by register tiles of 4 x 4, the
+// softmax with a running maximum and sum, values by tiles of 8 rows x 4 columns a thread. It is bound by the FMA pipe where
+// a step has 32 rows a kv head and by the copies through registers where it has few.
+#include "tree_plan.cuh"
+
+#define TA_THREADS 128
+#define TA_ROWS 32
+#define TA_PROW 36                // numbers a key's row of weights takes in shared memory
+
+struct TreeArgs {
+    const void* q;
+    const void* kcache;
+    const void* vcache;
+    const int* block_table;
+    const int* cu_q;
+    const int* seq_start;
+    const int* tok_pos;
+    const unsigned long long* mask;
+    void* out;
+    float* part_o;                // [pairs][nq][dv]
+    float2* part_ml;              // [pairs][nq]: running maximum and sum
+    const float* sink;
+    int bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec;
+    float scale, softcap;
+};
+
+// the denominator's reciprocal for sums whose reference is m (natural units), beside the sink's term; rescales by `f`
+__device__ __forceinline__ float ta_close(float m, float l, const float* sink, int head) {
+    if (m == -INFINITY) return l == 0.0f ? 0.0f : l;        // no weight at all, or a score that is no number
+    if (!sink) return 1.0f / l;
+    const float s = sink[head], top = fmaxf(m, s), f = expf(m - top);
+    return f / (l * f + expf(s - top));
+}
+
+// A page tile of `cols` numbers a row, into rows of `stride` float32 (columns up to `pad` zero); rows from `valid` on are zero.
+// Returns whether a number that is not finite was among this thread's.
+template <typename T>
+__device__ __forceinline__ bool ta_stage(float* dst, int stride, int pad, const T* tile, int cols, int layout, int valid, int vec) {
+    bool bad = false;
+    if (vec) {
+        constexpr int E = 16 / (int)sizeof(T);
+        const int pieces = cols / E, padded = pad / E;
+        for (int idx = threadIdx.x; idx < LUMEN_PAGE * padded; idx += TA_THREADS) {
+            const int r = idx / padded, c = idx - r * padded;
+            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+            if (r < valid && c < pieces) raw = *reinterpret_cast<const uint4*>(tile + tile_offset(layout, r, c * E, cols));
+            const T* x = reinterpret_cast<const T*>(&raw);
+            float f[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                f[i] = to_f32(x[i]);
+                bad |= !(fabsf(f[i]) <= 3.402823466e38f);
+            }
+#pragma unroll
+            for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(dst + r * stride + c * E + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        }
+    } else {
+        for (int idx = threadIdx.x; idx < LUMEN_PAGE * pad; idx += TA_THREADS) {
+            const int r = idx / pad, e = idx - r * pad;
+            const float f = (r < valid && e < cols) ? to_f32(tile[tile_offset(layout, r, e, cols)]) : 0.0f;
+            bad |= !(fabsf(f) <= 3.402823466e38f);
+            dst[r * stride + e] = f;
+        }
+    }
+    return bad;
+}
+
+template <typename T, int NC>
+__global__ void __launch_bounds__(TA_THREADS)
+attn_tree_kernel(const TreeArgs a) {
+    pdl_wait();      // nothing of this kernel touches global memory before this
+    pdl_trigger();
+    extern __shared__ __align__(16) float ta_smem[];
+    __shared__ float s_corr[TA_ROWS], s_inv[TA_ROWS];
+    __shared__ int s_unit[2];
+    const int G = a.nq / a.nkv, tid = threadIdx.x;
+    const int kvh = blockIdx.x % a.nkv, seg = blockIdx.y;
+    if (tid < 32) {
+        int b, tile;
+        tree_find(a.cu_q, a.B, a.N, G, TA_ROWS, blockIdx.x / a.nkv, b, tile);
+        if (tid == 0) { s_unit[0] = b; s_unit[1] = tile; }
+    }
+    __syncthreads();
+    const int b = s_unit[0];
+    if (b >= a.B) return;
+    const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, b, a.N, a.width);
+    const TreePlan plan = tree_plan(sq, a.window, G);
+    if (seg >= plan.nseg) return;
+    const int f0 = s_unit[1] * TA_ROWS, nrows = min(TA_ROWS, sq.q * G - f0);
+    const int dp = (a.d + 3) & ~3, ks = dp + 4;
+    float* qs = ta_smem;                          // [32][ks]
+    float* kv = qs + TA_ROWS * ks;                // [64][ks] keys, then [64][128 NC] values
+    float* ps = kv + LUMEN_PAGE * max(ks, 128 * NC);      // [64][TA_PROW]: weights, a key's rows together
+    const T* q = (const T*)a.q;
+
+    for (int idx = tid; idx < TA_ROWS * dp; idx += TA_THREADS) {
+        const int r = idx / dp, e = idx - r * dp, f = f0 + r;
+        qs[r * ks + e] = (r < nrows && e < a.d) ? to_f32(q[((size_t)(sq.n0 + f / G) * a.nq + kvh * G + f % G) * a.d + e]) : 0.0f;
+    }
+    // scores: rows 4 rg .. 4 rg + 3, keys kg, kg + 16, kg + 32, kg + 48
+    const int rg = tid >> 4, kg = tid & 15;
+    const unsigned long long* mask[4];
+    int pos[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = sq.n0 + (f0 + min(4 * rg + i, nrows - 1)) / G;
+        mask[i] = a.mask + (size_t)n * a.W;
+        pos[i] = max(a.tok_pos[n], sq.start);
+    }
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // values: rows 8 wr .. 8 wr + 7, columns 4 lane + 128 c .. + 3
+    const int wr = tid >> 5, lane = tid & 31;
+    float acc[8][4 * NC];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int c = 0; c < 4 * NC; ++c) acc[r][c] = 0.0f;
+    const int* bt = a.block_table + (size_t)b * a.bt_stride;
+
+    for (int pg = plan.first(seg), last = pg + plan.count(seg); pg < last; ++pg) {
+        int page = bt[pg];
+        if ((unsigned)page >= (unsigned)a.n_pages) page = 0;
+        const size_t tile = (size_t)page * a.nkv + kvh;
+        const int jb = pg * LUMEN_PAGE, valid = min(LUMEN_PAGE, sq.end - jb);
+        __syncthreads();
+        ta_stage<T>(kv, ks, dp, (const T*)a.kcache + tile * (size_t)(LUMEN_PAGE * a.d), a.d, a.layout, valid, a.vec & 1);
+        __syncthreads();
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[i][k] = 0.0f;
+        for (int e = 0; e < dp; e += 4) {
+            float4 x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(qs + (4 * rg + i) * ks + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const float4*>(kv + (kg + 16 * k) * ks + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s[i][k] = fmaf(x[i].x, y[k].x, s[i][k]);
+                    s[i][k] = fmaf(x[i].y, y[k].y, s[i][k]);
+                    s[i][k] = fmaf(x[i].z, y[k].z, s[i][k]);
+                    s[i][k] = fmaf(x[i].w, y[k].w, s[i][k]);
+                }
+        }
+        float corr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned long long seen = tree_seen(jb, sq, mask[i], a.W, pos[i], a.window, a.tok_pos + sq.n0);
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float x = s[i][k] * a.scale;
+                if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+                s[i][k] = (seen >> (kg + 16 * k)) & 1 ? x : -INFINITY;
+                top = fmaxf(top, s[i][k]);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float mn = fmaxf(m[i], top), base = mn == -INFINITY ? 0.0f : mn;
+            corr[i] = m[i] == -INFINITY ? 0.0f : expf(m[i] - mn);
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s[i][k] = expf(s[i][k] - base);      // 0 for a masked key, also where none has been seen yet
+                sum += s[i][k];
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[i] = l[i] * corr[i] + sum;
+            m[i] = mn;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(ps + (kg + 16 * k) * TA_PROW + 4 * rg) = make_float4(s[0][k], s[1][k], s[2][k], s[3][k]);
+        if (kg == 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_corr[4 * rg + i] = corr[i];
+        __syncthreads();                          // the keys have been read, the weights are there
+        const bool bad = ta_stage<T>(kv, 128 * NC, 128 * NC, (const T*)a.vcache + tile * (size_t)(LUMEN_PAGE * a.dv), a.dv, a.v_layout,
+                                     valid, a.vec & 2);
+        const bool any_bad = __syncthreads_or(bad);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float c = s_corr[8 * wr + r];
+#pragma unroll
+            for (int x = 0; x < 4 * NC; ++x) acc[r][x] *= c;
+        }
+        for (int k = 0; k < valid; ++k) {
+            float w[8];
+            *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(ps + k * TA_PROW + 8 * wr);
+            *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(ps + k * TA_PROW + 8 * wr + 4);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float4 v = *reinterpret_cast<const float4*>(kv + k * (128 * NC) + 128 * c + 4 * lane);
+                if (any_bad) {                    // nothing of a masked value, not even 0 times infinity
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (w[r] != 0.0f) {
+                            acc[r][4 * c] = fmaf(w[r], v.x, acc[r][4 * c]);
+                            acc[r][4 * c + 1] = fmaf(w[r], v.y, acc[r][4 * c + 1]);
+                            acc[r][4 * c + 2] = fmaf(w[r], v.z, acc[r][4 * c + 2]);
+                            acc[r][4 * c + 3] = fmaf(w[r], v.w, acc[r][4 * c + 3]);
+                        }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        acc[r][4 * c] = fmaf(w[r], v.x, acc[r][4 * c]);
+                        acc[r][4 * c + 1] = fmaf(w[r], v.y, acc[r][4 * c + 1]);
+                        acc[r][4 * c + 2] = fmaf(w[r], v.z, acc[r][4 * c + 2]);
+                        acc[r][4 * c + 3] = fmaf(w[r], v.w, acc[r][4 * c + 3]);
+                    }
+                }
+            }
+        }
+    }
+    const bool whole = plan.nseg == 1;
+    const long long pair0 = tree_part_base(b, sq.n0, a.width, G);
+    if (kg == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * rg + i, f = f0 + r;
+            if (r >= nrows) continue;
+            const int head = kvh * G + f % G;
+            if (whole) s_inv[r] = ta_close(m[i], l[i], a.sink, head);
+            else a.part_ml[(pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head] = make_float2(m[i], l[i]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int row = 8 * wr + r, f = f0 + row;
+        if (row >= nrows) continue;
+        const int head = kvh * G + f % G;
+        if (whole) {
+            T* dst = (T*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv;
+            const float inv = s_inv[row];
+#pragma unroll
+            for (int c = 0; c < 4 * NC; ++c) {
+                const int e = 4 * lane + 128 * (c >> 2) + (c & 3);
+                if (e < a.dv) dst[e] = from_f32<T>(acc[r][c] * inv);
+            }
+        } else {
+            float* dst = a.part_o + ((pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head) * (long long)a.dv;
+#pragma unroll
+            for (int c = 0; c < 4 * NC; ++c) {
+                const int e = 4 * lane + 128 * (c >> 2) + (c & 3);
+                if (e < a.dv) dst[e] = acc[r][c];
+            }
+        }
+    }
+}
+
+// Joins the segments of the sequences that have more than one, in rising order: a thread has four columns of a (token, head).
+// BASE2: the partial maxima are in units of log 2 (the tensor-core kernel's).
+template <typename T, bool BASE2>
+__global__ void __launch_bounds__(128)
+attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
+    pdl_wait();
+    pdl_trigger();
+    const int n = blockIdx.x, b = tok_seq[n];
+    if ((unsigned)b >= (unsigned)a.B) return;
+    const int G = a.nq / a.nkv;
+    const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, b, a.N, a.width);
+    if (n < sq.n0 || n >= sq.n0 + sq.q) return;
+    const TreePlan plan = tree_plan(sq, a.window, G);
+    if (plan.nseg == 1) return;                   // done by its own block
+    const int quads = (a.dv + 3) / 4, idx = blockIdx.y * 128 + threadIdx.x;
+    if (idx >= a.nq * quads) return;
+    const int head = idx / quads, e = (idx - head * quads) * 4;
+    const long long pair = tree_part_base(b, sq.n0, a.width, G) + (long long)(n - sq.n0) * plan.nseg;
+    const float2* ml = a.part_ml + pair * a.nq + head;
+    float top = -INFINITY;
+    for (int s = 0; s < plan.nseg; ++s) top = fmaxf(top, ml[(long long)s * a.nq].x);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+    for (int s = 0; s < plan.nseg; ++s) {
+        const float2 x = ml[(long long)s * a.nq];
+        if (x.x == -INFINITY && x.y == 0.0f) continue;      // no key of that segment is in the row's sight
+        const float f = BASE2 ? exp2f(x.x - top) : expf(x.x - top);
+        const float* p = a.part_o + ((pair + s) * a.nq + head) * (long long)a.dv + e;
+        float v[4];
+        if ((a.dv & 3) == 0) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+        else
+            for (int i = 0; i < 4; ++i) v[i] = e + i < a.dv ? p[i] : 0.0f;
+        o.x = fmaf(f, v[0], o.x); o.y = fmaf(f, v[1], o.y); o.z = fmaf(f, v[2], o.z); o.w = fmaf(f, v[3], o.w);
+        l = fmaf(f, x.y, l);
+    }
+    const float inv = ta_close(BASE2 ? top * 0.6931471805599453f : top, l, a.sink, head);
+    T* dst = (T*)a.out + ((size_t)n * a.nq + head) * a.dv + e;
+    const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    for (int i = 0; i < 4; ++i)
+        if (e + i < a.dv) dst[i] = from_f32<T>(v[i]);
+}
+
+template <typename T>
+static cudaError_t ta_join(const TreeArgs& a, const int* tok_seq, int base2, cudaStream_t stream) {
+    const dim3 grid(a.N, ((a.dv + 3) / 4 * a.nq + 127) / 128);
+    return base2 ? lumen_launch(attn_tree_join_kernel<T, true>, grid, dim3(128), 0, stream, a, tok_seq)
+                 : lumen_launch(attn_tree_join_kernel<T, false>, grid, dim3(128), 0, stream, a, tok_seq);
+}
+
+template <typename T, int NC>
+static cudaError_t ta_go(const TreeArgs& a, int max_segs, cudaStream_t stream) {
+    const int ks = ((a.d + 3) & ~3) + 4, wide = ks > 128 * NC ? ks : 128 * NC;
+    const int smem = (TA_ROWS * ks + LUMEN_PAGE * wide + LUMEN_PAGE * TA_PROW) * (int)sizeof(float);
+    auto k = attn_tree_kernel<T, NC>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)a.N * (a.nq / a.nkv) / TA_ROWS + a.B;
+    return lumen_launch(k, dim3((unsigned)(tiles * a.nkv), max_segs), dim3(TA_THREADS), smem, stream, a);
+}
+
+// Segments that a page table of `width` pages may be cut into.
+static int ta_segs(int width) {
+    const int n = (width + TREE_MIN_SEG - 1) / TREE_MIN_SEG;
+    return n < TREE_MAX_SEGS ? n : TREE_MAX_SEGS;
+}
+
+// q [N, nq, d], out [N, nq, dv] in the cache's type; keys [n_pages, nkv, 64, d], values [n_pages, nkv, 64, dv]; mask
+// [N, W] 64-bit words. Where width is above TREE_MIN_SEG sequences may be cut: parts then is float32 [pairs, nq, 2 + dv] for
+// pairs >= B tree_part_room(width, nq / nkv) + N, an even number.
+LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vcache, const int* block_table, int bt_stride,
+                              int width, const int* cu_q, const int* seq_start, const int* tok_seq, const int* tok_pos,
+                              const void* mask, int W, void* out, float* parts, long long pairs, int is_bf16, int B, int N,
+                              int n_pages, int nq, int nkv, int d, int dv, int window, float scale, float softcap,
+                              const float* sink, int layout, int v_layout, cudaStream_t stream) {
+    if (B <= 0 || N <= 0) return 0;
+    if (nq <= 0 || nkv <= 0 || nq % nkv || d <= 0 || d > 512 || dv <= 0 || dv > 512 || window < 0 || softcap < 0.0f || W < 1 ||
+        width < 1 || width > (1 << 24) || n_pages < 1)
+        return LUMEN_ERR_UNSUPPORTED;
+    if ((layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || d % 64)) || (v_layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || dv % 64)))
+        return LUMEN_ERR_UNSUPPORTED;
+    const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = ta_segs(width);
+    if (((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
+    if (max_segs > 1 && (!parts || (pairs & 1) || pairs < (long long)B * tree_part_room(width, G) + N)) return LUMEN_ERR_BAD_ARGUMENT;
+    float* part_o = parts ? parts + pairs * nq * 2 : nullptr;        // 16-byte rows where dv is a multiple of 4
+    const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0);
+    const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out, part_o,
+                        (float2*)parts, sink, bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec,
+                        scale, softcap};
+    cudaError_t e;
+#define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, max_segs, stream) : ta_go<T, 4>(a, max_segs, stream))
+    e = is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
+#undef TA_GO
+    if (e != cudaSuccess) return (int)e;
+    if (max_segs > 1) {
+        e = is_bf16 ? ta_join<__nv_bfloat16>(a, tok_seq, 0, stream) : ta_join<float>(a, tok_seq, 0, stream);
+        if (e != cudaSuccess) return (int)e;
+    }
+    LUMEN_LAUNCH_CHECK();
+    return 0;
+}

@@ -7,6 +7,7 @@ in front, [S, rows, width]; the consumers below add the partials while reading.
 """
 from __future__ import annotations
 
+from collections import namedtuple
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -18,6 +19,7 @@ P = c_void_p
 F32 = torch.float32
 BF16 = torch.bfloat16
 I32 = torch.int32
+I64 = torch.int64
 
 PAGE = _page_size()   # tokens per cache page: LUMEN_PAGE of csrc/common.cuh
 LAYOUT_LINEAR, LAYOUT_SW128 = 0, 1   # tile layouts of the cache, as in csrc/common.cuh
@@ -1949,3 +1951,187 @@ def attn_prefill(q, kcache, vcache, block_table, cu_q, seq_start, q_lens, window
             ptr(seq_start), B, n_tiles, ptr(out), nq, nkv, d, int(window), float(scale),
             ptr(error_flag(q.device)), stream_ptr()), "attn_prefill")
     return out
+
+
+# ------------------------------------------------------------------ trees of drafted tokens
+
+TREE_MAX_NODES = 256      # nodes of a sequence that masks and walks cover: TREE_MAX_NODES of csrc/tree_plan.cuh
+TREE_MIN_SEG = 4          # pages of a page table that no sequence is cut in: TREE_MIN_SEG there
+
+StepTables = namedtuple("StepTables", "cu_q tok_seq cache_pos tok_pos slot_map block_table tree_mask")
+
+
+def _arrays(what, **tensors):
+    """Contiguous arrays of one type each, all on the current device: name=(tensor, dtype, numbers at least)."""
+    for name, (t, dtype, n) in tensors.items():
+        if t.dtype != dtype:
+            raise KernelError(f"{what}.{name}: expected {dtype}, got {t.dtype}")
+        if t.numel() < n:
+            raise KernelError(f"{what}.{name}: {t.numel()} numbers, {n} are needed")
+        if not t.is_contiguous():
+            raise KernelError(f"{what}.{name}: tensor must be contiguous")
+    _here(what, [t for t, _, _ in tensors.values()])
+
+
+def _here(what, tensors):
+    """All on a CUDA device, and on the current one (whose stream a launch goes to)."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError(f"{what}: a tensor is not on a CUDA device (no CPU path exists)")
+        if t.get_device() != torch.cuda.current_device():
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _page_table(what, block_table, rows):
+    if block_table.dim() != 2 or block_table.shape[0] < rows or block_table.shape[1] < 1 or block_table.dtype != I32 \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise KernelError(f"{what}.block_table: int32 [{rows} or more, pages] with dense rows is needed, not "
+                          f"{tuple(block_table.shape)} of {block_table.dtype}")
+
+
+def step_tables(seq_start, seq_qlen, slot_pages, seq_slot, n_tokens, width, parents=None, mask_words=1):
+    """The arrays of a step from its requests' lengths, made on the device: sequence b has seq_start[b] cached tokens
+    (int32 [B]), brings seq_qlen[b] (int32 [B]) and holds the pages of row seq_slot[b] (int32 [B]) of slot_pages (int32
+    [slots, at least `width`], rows dense). Returns StepTables: cu_q int32 [B + 1], tok_seq, cache_pos and tok_pos int32
+    [n_tokens], slot_map int64 [n_tokens] (page * PAGE + place of a token's key), block_table int32 [B + 1, width] (the pages a
+    sequence needs with its new tokens, zeros behind them; the last row all zeros), tree_mask.
+    Without `parents` a sequence's tokens follow one another: tok_pos is cache_pos, tree_mask None. With parents int32
+    [n_tokens] (of a token: the number of an earlier one of its sequence in this step; anything else stands for the last
+    cached token) a token's tok_pos is the sequence's cached length plus its depth, and tree_mask int64 [n_tokens,
+    mask_words] has bit t of word w where token 64 w + t of the sequence is the token itself or an ancestor.
+    Lengths are taken as far as there is room: tokens behind the page table's end (width * PAGE), behind 64 * mask_words of a
+    tree (mask_words up to 4) and behind n_tokens in all are left out, and lengths below 0 are 0. A slot outside slot_pages
+    has the page table row of zeros (page 0 takes the writes of padding). Tokens behind the last sequence have tok_seq B
+    (which is the table's last row), positions 0, slot_map -1 and an empty mask."""
+    B, N, width, words = seq_start.numel(), int(n_tokens), int(width), int(mask_words)
+    if slot_pages.dim() != 2 or slot_pages.dtype != I32 or slot_pages.shape[1] < width or (slot_pages.shape[1] > 1 and slot_pages.stride(1) != 1):
+        raise KernelError(f"step_tables.slot_pages: int32 [slots, {width} or more] with dense rows is needed, not "
+                          f"{tuple(slot_pages.shape)} of {slot_pages.dtype}")
+    if N < 0 or not 1 <= width <= 1 << 24 or not 1 <= words <= TREE_MAX_NODES // 64:
+        raise KernelError(f"step_tables: {N} tokens, {width} pages, {words} mask words")
+    _arrays("step_tables", seq_start=(seq_start, I32, B), seq_qlen=(seq_qlen, I32, B), seq_slot=(seq_slot, I32, B),
+            parents=(seq_start if parents is None else parents, I32, 0 if parents is None else N))
+    _here("step_tables", [slot_pages])
+    dev = seq_start.device
+    cu_q, tok_seq, cache_pos, tok_pos, table = torch.empty((B + 1 + 3 * N + (B + 1) * width,), dtype=I32, device=dev).split(
+        (B + 1, N, N, N, (B + 1) * width))
+    table = table.view(B + 1, width)
+    slot_map = torch.empty((N,), dtype=I64, device=dev)
+    mask = torch.empty((N, words), dtype=I64, device=dev) if parents is not None else None
+    f = fn("draft", "lumen_step_tables", [P, P, P, c_longlong, c_int, P, P, c_int, c_int, c_int, c_int, P, P, P, P, P, P, P, P])
+    check(f(ptr(seq_start), ptr(seq_qlen), ptr(slot_pages), slot_pages.stride(0), slot_pages.shape[0], ptr(seq_slot), ptr(parents),
+            B, N, width, words, ptr(cu_q), ptr(tok_seq), ptr(cache_pos), ptr(tok_pos), ptr(slot_map), ptr(table), ptr(mask),
+            stream_ptr()), "step_tables")
+    return StepTables(cu_q, tok_seq, cache_pos, tok_pos, slot_map, table, mask)
+
+
+def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos, tree_mask, window, scale,
+              layout=LAYOUT_LINEAR, v_layout=None, softcap=0.0, sink=False, out=None):
+    """Attention of a step whose sequences bring trees of drafted tokens, over the paged cache that holds their keys and values
+    already: q [N, nq, d]; keys [pages, nkv, PAGE, d]; values [pages, nkv, PAGE, dv]; returns [N, nq, dv] in q's type
+    (float32 or bfloat16, the cache's). cu_q int32 [B + 1] divides the tokens into sequences, tok_seq int32 [N] says the same
+    from the token's side; sequence b has seq_start[b] cached tokens, token i of it lies at index seq_start[b] + i of its cache
+    (page table row b). A token sees the cached tokens and those tokens m of its sequence whose bit m is set in its row of
+    tree_mask (int64 [N, W], W up to 4; any pattern; step_tables makes the ancestors'); with a window w > 0 only what
+    stands fewer than w positions before its own position tok_pos (int32 [N]; at least seq_start[b], where a cached token's
+    position is its index). Scores are scale * q . k, with softcap c > 0 then c tanh(score / c); `sink` (float32 [nq], or True for
+    zeros) adds exp(sink[head]) to the softmax's denominator. A row that sees nothing is 0. What a masked key or value holds does
+    not matter, infinities and NaN included. Rows behind the last sequence (cu_q[B]) are not written; `out` takes the result.
+    Keys and values up to 512 numbers, any nq that is a multiple of nkv."""
+    N, nq, d = q.shape
+    if q.dtype not in (F32, BF16) or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+        raise KernelError(f"attn_tree: queries and caches are all float32 or all bfloat16, not {q.dtype}, {kcache.dtype}, {vcache.dtype}")
+    if kcache.dim() != 4 or vcache.dim() != 4:
+        raise KernelError("attn_tree: caches are [pages, kv heads, PAGE, size]")
+    n_pages, nkv, dv = kcache.shape[0], kcache.shape[1], vcache.shape[3]
+    v_layout = layout if v_layout is None else v_layout
+    if tuple(kcache.shape[1:]) != (nkv, PAGE, d) or tuple(vcache.shape[:3]) != (n_pages, nkv, PAGE) or not nkv or nq % nkv or not nq:
+        raise KernelError(f"attn_tree: caches {tuple(kcache.shape)}, {tuple(vcache.shape)} do not fit {nq} queries of {d}")
+    if not 1 <= d <= 512 or not 1 <= dv <= 512 or n_pages < 1:
+        raise KernelError(f"attn_tree takes keys and values of 1 to 512 numbers, not {d} and {dv}")
+    for lay, size, nm in ((layout, d, "keys"), (v_layout, dv, "values")):
+        if lay not in (LAYOUT_LINEAR, LAYOUT_SW128) or (lay == LAYOUT_SW128 and (q.dtype != BF16 or size % 64)):
+            raise KernelError(f"attn_tree: {nm} of {size} numbers of {q.dtype} have no tile layout {lay}")
+    B = cu_q.numel() - 1
+    if tree_mask.dim() != 2 or not 1 <= tree_mask.shape[1] <= TREE_MAX_NODES // 64:
+        raise KernelError(f"attn_tree.tree_mask: int64 [{N}, 1 to {TREE_MAX_NODES // 64}] is needed, not {tuple(tree_mask.shape)}")
+    if window < 0 or not softcap >= 0.0 or B < 0:
+        raise KernelError(f"attn_tree: window {window}, softcap {softcap}, {B} sequences")
+    _page_table("attn_tree", block_table, B)
+    words = tree_mask.shape[1]
+    _arrays("attn_tree", q=(q, q.dtype, 0), kcache=(kcache, q.dtype, 0), vcache=(vcache, q.dtype, 0), cu_q=(cu_q, I32, 1),
+            seq_start=(seq_start, I32, B), tok_seq=(tok_seq, I32, N), tok_pos=(tok_pos, I32, N), tree_mask=(tree_mask, I64, N * words))
+    _here("attn_tree", [block_table])
+    if out is None:
+        out = torch.empty((N, nq, dv), dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (N, nq, dv):
+        raise KernelError(f"attn_tree: out {tuple(out.shape)} is not {(N, nq, dv)}")
+    else:
+        _arrays("attn_tree", out=(out, q.dtype, 0))
+    if N == 0 or B == 0:
+        return out
+    sink = _sink_arg(sink, nq, q.device)
+    width = block_table.shape[1]
+    # (token, segment) pairs of partial results: what csrc/tree_plan.cuh can come to, whatever the lengths are
+    pairs = (B * -(-8 * width // (nq // nkv)) + N + 1) // 2 * 2 if width > TREE_MIN_SEG else 0
+    parts = torch.empty((pairs * nq * (dv + 2),), dtype=F32, device=q.device) if pairs else None
+    f = fn("attn_tree", "lumen_attn_tree",
+           [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, P, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+            c_int, c_float, c_float, P, c_int, c_int, P])
+    check(f(ptr(q), ptr(kcache), ptr(vcache), ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq),
+            ptr(tok_pos), ptr(tree_mask), words, ptr(out), ptr(parts), pairs, _is_bf16(q), B, N, n_pages, nq, nkv, d, dv, int(window),
+            float(scale), float(softcap), ptr(sink), int(layout), int(v_layout), stream_ptr()), "attn_tree")
+    return out
+
+
+def tree_accept(picked, tokens, parents, cu_q, max_path):
+    """Which drafted tokens a model agrees with: picked, tokens, parents int32 [N], cu_q int32 [B + 1]. picked[n] is what the
+    model answers at token n; the walk through sequence b begins at its first token (which is certain) and goes on to the
+    child whose token is the one picked at its parent (the lowest of several), as long as there is one and the path has room.
+    parents as in step_tables. Returns (count int32 [B], path int32 [B, max_path], emitted int32 [B, max_path]): the
+    tokens on the path (0 for a sequence without tokens), their numbers in the sequence and what was picked at each (the
+    sequence's next `count` tokens), -1 behind them. max_path up to 256; a sequence's tokens behind its first 256 are not
+    walked."""
+    N, B, most = picked.numel(), cu_q.numel() - 1, int(max_path)
+    if B < 0 or not 1 <= most <= TREE_MAX_NODES:
+        raise KernelError(f"tree_accept: {B} sequences, paths of up to {max_path} (1 to {TREE_MAX_NODES})")
+    _arrays("tree_accept", picked=(picked, I32, N), tokens=(tokens, I32, N), parents=(parents, I32, N), cu_q=(cu_q, I32, 1))
+    count, path, emitted = torch.empty((B * (1 + 2 * most),), dtype=I32, device=picked.device).split((B, B * most, B * most))
+    f = fn("draft", "lumen_tree_accept", [P, P, P, P, c_int, c_int, c_int, P, P, P, P])
+    check(f(ptr(picked), ptr(tokens), ptr(parents), ptr(cu_q), B, N, most, ptr(count), ptr(path), ptr(emitted), stream_ptr()),
+          "tree_accept")
+    return count, path.view(B, most), emitted.view(B, most)
+
+
+def cache_compact(kcache, vcache, block_table, seq_start, path, count, layout=LAYOUT_LINEAR, v_layout=None):
+    """Moves the accepted tokens' rows to where the next step expects them: for every sequence b the keys and values at index
+    seq_start[b] + path[b, k] of its cache go to index seq_start[b] + k, for k = 1 .. count[b] - 1, in place, in every
+    layer. kcache [pages, nkv, PAGE, d] or [layers, pages, nkv, PAGE, d], vcache as many of its own width (None: keys alone;
+    float32 or bfloat16); block_table int32 [B or more, pages a sequence]; seq_start, count int32 [B]; path int32 [B, most], as
+    tree_accept gives it: rising numbers. A path ends before a number that is not above the one before it, lies behind the page
+    table, or is on a page that the cache has not; sequences must not share the pages that are written."""
+    shape = tuple(kcache.shape)
+    if kcache.dim() not in (4, 5) or shape[-2] != PAGE or kcache.dtype not in (F32, BF16) or 0 in shape[-4:]:
+        raise KernelError(f"cache_compact: keys are float32 or bfloat16 [layers, pages, kv heads, {PAGE}, size], not {shape} of {kcache.dtype}")
+    layers, n_pages, nkv, d = (shape[0] if len(shape) == 5 else 1), shape[-4], shape[-3], shape[-1]
+    dv = 0
+    if vcache is not None:
+        dv = vcache.shape[-1]
+        if tuple(vcache.shape[:-1]) != shape[:-1] or vcache.dtype != kcache.dtype or not dv:
+            raise KernelError(f"cache_compact: values {tuple(vcache.shape)} of {vcache.dtype} do not fit keys {shape}")
+    v_layout = layout if v_layout is None else v_layout
+    for lay, size in ((layout, d),) + (((v_layout, dv),) if vcache is not None else ()):
+        if lay not in (LAYOUT_LINEAR, LAYOUT_SW128) or (lay == LAYOUT_SW128 and (kcache.dtype != BF16 or size % 64)):
+            raise KernelError(f"cache_compact: rows of {size} numbers of {kcache.dtype} have no tile layout {lay}")
+    B = count.numel()
+    if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= TREE_MAX_NODES or B > 65535 or n_pages > 1 << 24:
+        raise KernelError(f"cache_compact: path {tuple(path.shape)} for {B} sequences (1 to {TREE_MAX_NODES} tokens each)")
+    _page_table("cache_compact", block_table, B)
+    _arrays("cache_compact", kcache=(kcache, kcache.dtype, 0), vcache=(kcache if vcache is None else vcache, kcache.dtype, 0),
+            seq_start=(seq_start, I32, B), path=(path, I32, 0), count=(count, I32, 0))
+    _here("cache_compact", [block_table])
+    f = fn("draft", "lumen_cache_compact", [P, P, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                            c_int, c_int, P])
+    check(f(ptr(kcache), ptr(vcache), ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(seq_start), ptr(path),
+            path.shape[1], ptr(count), B, layers, n_pages, nkv, d, dv, int(layout), int(v_layout), 4 if kcache.dtype == F32 else 2,
+            stream_ptr()), "cache_compact")
