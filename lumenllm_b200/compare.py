@@ -240,6 +240,9 @@ CLASSES = {
     "lumen_add_shaped_rmsnorm": "norm", "lumen_rglru": "recurrent unit: recurrence",
     "lumen_gemm_tc_blocks": "block-diagonal product", "lumen_block_product": "block-diagonal product",
     "lumen_shift_mix": "time mixing: token shift", "lumen_gemm_f32_tc": "float32 product",
+    "lumen_attn_tree": "attention", "lumen_step_tables": "trees of drafted tokens: tables, walk, cache move",
+    "lumen_tree_accept": "trees of drafted tokens: tables, walk, cache move",
+    "lumen_cache_compact": "trees of drafted tokens: tables, walk, cache move",
 }
 
 

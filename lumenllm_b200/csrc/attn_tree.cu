@@ -326,6 +326,8 @@ static cudaError_t ta_go(const TreeArgs& a, int max_segs, cudaStream_t stream) {
     return lumen_launch(k, dim3((unsigned)(tiles * a.nkv), max_segs), dim3(TA_THREADS), smem, stream, a);
 }
 
+#include "attn_tree_tc.cuh"
+
 // Segments that a page table of `width` pages may be cut into.
 static int ta_segs(int width) {
     const int n = (width + TREE_MIN_SEG - 1) / TREE_MIN_SEG;
@@ -339,7 +341,7 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
                               int width, const int* cu_q, const int* seq_start, const int* tok_seq, const int* tok_pos,
                               const void* mask, int W, void* out, float* parts, long long pairs, int is_bf16, int B, int N,
                               int n_pages, int nq, int nkv, int d, int dv, int window, float scale, float softcap,
-                              const float* sink, int layout, int v_layout, cudaStream_t stream) {
+                              const float* sink, int layout, int v_layout, int* err, cudaStream_t stream) {
     if (B <= 0 || N <= 0) return 0;
     if (nq <= 0 || nkv <= 0 || nq % nkv || d <= 0 || d > 512 || dv <= 0 || dv > 512 || window < 0 || softcap < 0.0f || W < 1 ||
         width < 1 || width > (1 << 24) || n_pages < 1)
@@ -354,13 +356,14 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out, part_o,
                         (float2*)parts, sink, bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec,
                         scale, softcap};
+    const bool tc = tt_takes(a, is_bf16);
     cudaError_t e;
 #define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, max_segs, stream) : ta_go<T, 4>(a, max_segs, stream))
-    e = is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
+    e = tc ? tt_launch(a, max_segs, err, stream) : is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
 #undef TA_GO
     if (e != cudaSuccess) return (int)e;
     if (max_segs > 1) {
-        e = is_bf16 ? ta_join<__nv_bfloat16>(a, tok_seq, 0, stream) : ta_join<float>(a, tok_seq, 0, stream);
+        e = is_bf16 ? ta_join<__nv_bfloat16>(a, tok_seq, tc, stream) : ta_join<float>(a, tok_seq, 0, stream);
         if (e != cudaSuccess) return (int)e;
     }
     LUMEN_LAUNCH_CHECK();

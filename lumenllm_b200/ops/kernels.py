@@ -2077,10 +2077,10 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
     parts = torch.empty((pairs * nq * (dv + 2),), dtype=F32, device=q.device) if pairs else None
     f = fn("attn_tree", "lumen_attn_tree",
            [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, P, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-            c_int, c_float, c_float, P, c_int, c_int, P])
+            c_int, c_float, c_float, P, c_int, c_int, P, P])
     check(f(ptr(q), ptr(kcache), ptr(vcache), ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq),
             ptr(tok_pos), ptr(tree_mask), words, ptr(out), ptr(parts), pairs, _is_bf16(q), B, N, n_pages, nq, nkv, d, dv, int(window),
-            float(scale), float(softcap), ptr(sink), int(layout), int(v_layout), stream_ptr()), "attn_tree")
+            float(scale), float(softcap), ptr(sink), int(layout), int(v_layout), ptr(error_flag(q.device)), stream_ptr()), "attn_tree")
     return out
 
 
