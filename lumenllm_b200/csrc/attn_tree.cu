@@ -349,7 +349,7 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     if ((layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || d % 64)) || (v_layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || dv % 64)))
         return LUMEN_ERR_UNSUPPORTED;
     const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = ta_segs(width);
-    if (((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
+    if (((long long)N * G / TA_ROWS + B) * nkv * max_segs > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
     if (max_segs > 1 && (!parts || (pairs & 1) || pairs < (long long)B * tree_part_room(width, G) + N)) return LUMEN_ERR_BAD_ARGUMENT;
     float* part_o = parts ? parts + pairs * nq * 2 : nullptr;        // 16-byte rows where dv is a multiple of 4
     const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0);
