@@ -266,6 +266,11 @@ attn_tree_kernel(const TreeArgs a) {
     }
 }
 
+__device__ __forceinline__ unsigned ta_pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+
 // Joins the segments of the sequences that have more than one, in rising order: a thread has four columns of a (token, head).
 // BASE2: the partial maxima are in units of log 2 (the tensor-core kernel's).
 template <typename T, bool BASE2>
@@ -285,25 +290,55 @@ attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
     const int head = idx / quads, e = (idx - head * quads) * 4;
     const long long pair = tree_part_base(b, sq.n0, a.width, G) + (long long)(n - sq.n0) * plan.nseg;
     const float2* ml = a.part_ml + pair * a.nq + head;
-    float top = -INFINITY;
-    for (int s = 0; s < plan.nseg; ++s) top = fmaxf(top, ml[(long long)s * a.nq].x);
+    const float* src = a.part_o + (pair * a.nq + head) * (long long)a.dv + e;
+    const long long row = (long long)a.nq * a.dv;
+    const bool quad = (a.dv & 3) == 0, quad_out = quad && ((uintptr_t)a.out & 7) == 0;
+    // one pass, a batch of segments at a time: their loads are under way together
+    constexpr int BATCH = 8;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-    for (int s = 0; s < plan.nseg; ++s) {
-        const float2 x = ml[(long long)s * a.nq];
-        if (x.x == -INFINITY && x.y == 0.0f) continue;      // no key of that segment is in the row's sight
-        const float f = BASE2 ? exp2f(x.x - top) : expf(x.x - top);
-        const float* p = a.part_o + ((pair + s) * a.nq + head) * (long long)a.dv + e;
-        float v[4];
-        if ((a.dv & 3) == 0) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-        else
-            for (int i = 0; i < 4; ++i) v[i] = e + i < a.dv ? p[i] : 0.0f;
-        o.x = fmaf(f, v[0], o.x); o.y = fmaf(f, v[1], o.y); o.z = fmaf(f, v[2], o.z); o.w = fmaf(f, v[3], o.w);
-        l = fmaf(f, x.y, l);
+    float l = 0.0f, top = -INFINITY;
+    for (int s0 = 0; s0 < plan.nseg; s0 += BATCH) {
+        float2 x[BATCH];
+        float4 v[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            x[i] = make_float2(-INFINITY, 0.0f);
+            v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s0 + i < plan.nseg) {
+                x[i] = ml[(long long)(s0 + i) * a.nq];
+                const float* p = src + (s0 + i) * row;
+                if (quad) v[i] = *reinterpret_cast<const float4*>(p);
+                else {
+                    v[i].x = p[0];
+                    if (e + 1 < a.dv) v[i].y = p[1];
+                    if (e + 2 < a.dv) v[i].z = p[2];
+                    if (e + 3 < a.dv) v[i].w = p[3];
+                }
+            }
+        }
+        float mn = top;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) mn = fmaxf(mn, x[i].x);
+        const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : BASE2 ? exp2f(top - mn) : expf(top - mn);
+        o.x *= c; o.y *= c; o.z *= c; o.w *= c;
+        l *= c;
+        top = mn;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;      // no key of that segment is in the row's sight
+            const float f = x[i].x == -INFINITY ? 1.0f : BASE2 ? exp2f(x[i].x - mn) : expf(x[i].x - mn);
+            o.x = fmaf(f, v[i].x, o.x); o.y = fmaf(f, v[i].y, o.y); o.z = fmaf(f, v[i].z, o.z); o.w = fmaf(f, v[i].w, o.w);
+            l = fmaf(f, x[i].y, l);
+        }
     }
     const float inv = ta_close(BASE2 ? top * 0.6931471805599453f : top, l, a.sink, head);
     T* dst = (T*)a.out + ((size_t)n * a.nq + head) * a.dv + e;
     const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    if (quad_out && sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(ta_pack(v[0], v[1]), ta_pack(v[2], v[3]));
+        return;
+    }
+#pragma unroll
     for (int i = 0; i < 4; ++i)
         if (e + i < a.dv) dst[i] = from_f32<T>(v[i]);
 }

@@ -37,6 +37,29 @@ struct TreeUnit {
 };
 #define TT_UNIT_INTS 11
 
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// A whole warp's wait (one lane asks) and question.
+__device__ __forceinline__ bool tt_warp_wait(uint64_t* bar, uint32_t parity) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ bool tt_warp_test(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); }
+// One lane of a whole warp, the same one every time.
+__device__ __forceinline__ bool tt_elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p)::"memory");
+    return p != 0;
+}
+
 // The units in order, found by a whole warp: lane i holds sequence b0 + i. Sequences in order; of one, segments, then kv
 // heads, then row tiles, so that tiles which read the same keys run side by side.
 struct TreeFinder {
@@ -125,7 +148,6 @@ attn_tree_tc_kernel(const TreeTc t) {
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_bad = reinterpret_cast<int*>(tmem_slot + 2);        // [2] unit number + 1 where a visible place of a masked page holds no number
     volatile int* s_unit = s_bad + 2;          // [2][TT_UNIT_INTS]
-    int* s_pos = s_bad + 2 + 2 * TT_UNIT_INTS; // [256] the nodes' positions
 
     const int G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -164,114 +186,118 @@ attn_tree_tc_kernel(const TreeTc t) {
         TreeFinder find;
         find.b0 = find.base = 0;
         find.chunk(a, G, lane);
-        int c = 0, v_asked = 0;                         // K and V tiles asked for
+        uint32_t ck = 0, cv = 0;                        // K and V tiles asked for
         bool ok = true;
-        const __nv_bfloat16* v_next = nullptr;          // the V tile of the page before: it is asked for behind the next K tile
-        auto ask_v = [&]() {                            // lane 0
-            const int st = v_asked % TT_STAGES;
-            if (!mbar_wait(&v_empty[st], ((v_asked / TT_STAGES) & 1) ^ 1)) return false;
-            mbar_expect_tx(&v_full[st], V_BYTES);
-            bulk_load(sKV + st * STAGE_BYTES + K_BYTES, v_next, V_BYTES, &v_full[st]);
-            ++v_asked;
-            return true;
-        };
         for (int k = 0, u = blockIdx.x; ok; ++k, u += gridDim.x) {
             const TreeUnit x = find.at(a, G, lane, u);
             const int slot = k & 1;
+            if (!(ok = tt_warp_wait(&u_empty[slot], ((k >> 1) & 1) ^ 1))) break;
             if (lane == 0) {
-                if (x.npages == 0 && c > 0) ok = ask_v();
-                ok = ok && mbar_wait(&u_empty[slot], ((k >> 1) & 1) ^ 1);
-                if (ok) {
-                    volatile int* to = s_unit + slot * TT_UNIT_INTS;
-                    to[0] = x.npages; to[1] = x.pg0; to[2] = x.b; to[3] = x.n0; to[4] = x.q; to[5] = x.start; to[6] = x.end;
-                    to[7] = x.f0; to[8] = x.kvh; to[9] = x.seg; to[10] = x.nseg;
-                    pt_mbar_arrive(&u_full[slot]);
-                }
+                volatile int* to = s_unit + slot * TT_UNIT_INTS;
+                to[0] = x.npages; to[1] = x.pg0; to[2] = x.b; to[3] = x.n0; to[4] = x.q; to[5] = x.start; to[6] = x.end;
+                to[7] = x.f0; to[8] = x.kvh; to[9] = x.seg; to[10] = x.nseg;
+                pt_mbar_arrive(&u_full[slot]);
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
             if (x.npages == 0) break;
             const int* bt = a.block_table + (size_t)x.b * a.bt_stride + x.pg0;
-            int ids = 0;
-            for (int i = 0; i < x.npages && ok; ++i) {
-                if ((i & 31) == 0) {
-                    ids = i + lane < x.npages ? bt[i + lane] : 0;
-                    if ((unsigned)ids >= (unsigned)a.n_pages) ids = 0;
-                }
-                const size_t tile = (size_t)__shfl_sync(0xffffffffu, ids, i & 31) * a.nkv + x.kvh;
-                if (lane == 0) {
-                    const int st = c % TT_STAGES;
-                    ok = !*abort_flag && mbar_wait(&k_empty[st], ((c / TT_STAGES) & 1) ^ 1);
-                    if (ok) {
+            const uint32_t first = cv, end = cv + x.npages;
+            int ids = 0, before = 0;                    // page numbers 32 at a time, and the ones before them
+            uint32_t spin = 0;
+            while (cv < end) {
+                // whichever slot is free: K tiles run ahead of V tiles, their slots come free earlier
+                if (ck < end && tt_warp_test(&k_empty[ck % TT_STAGES], ((ck / TT_STAGES) & 1) ^ 1)) {
+                    const uint32_t i = ck - first, st = ck % TT_STAGES;
+                    if ((i & 31) == 0) {
+                        before = ids;
+                        ids = (int)(i + lane) < x.npages ? bt[i + lane] : 0;
+                        if ((unsigned)ids >= (unsigned)a.n_pages) ids = 0;
+                    }
+                    const size_t tile = (size_t)__shfl_sync(0xffffffffu, ids, i & 31) * a.nkv + x.kvh;
+                    if (lane == 0) {
                         mbar_expect_tx(&k_full[st], K_BYTES);
                         bulk_load(sKV + st * STAGE_BYTES, kcache + tile * (size_t)(LUMEN_PAGE * kw), K_BYTES, &k_full[st]);
-                        if (c > 0) ok = ask_v();
-                        ++c;
-                        v_next = vcache + tile * (size_t)(LUMEN_PAGE * vw);
                     }
+                    ++ck;
+                    spin = 0;
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (cv < ck && tt_warp_test(&v_empty[cv % TT_STAGES], ((cv / TT_STAGES) & 1) ^ 1)) {
+                    const uint32_t i = cv - first, st = cv % TT_STAGES;
+                    const int from = (i >> 5) == ((ck - first - 1) >> 5) ? ids : before;
+                    const size_t tile = (size_t)__shfl_sync(0xffffffffu, from, i & 31) * a.nkv + x.kvh;
+                    if (lane == 0) {
+                        mbar_expect_tx(&v_full[st], V_BYTES);
+                        bulk_load(sKV + st * STAGE_BYTES + K_BYTES, vcache + tile * (size_t)(LUMEN_PAGE * vw), V_BYTES, &v_full[st]);
+                    }
+                    ++cv;
+                    spin = 0;
+                }
+                if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
             }
         }
         if (lane == 0 && !ok) {
             *abort_flag = 1;
             atomicExch(t.err, 1);
-            for (int i = max(0, c - TT_STAGES); i < c; ++i) mbar_wait(&k_full[i % TT_STAGES], (i / TT_STAGES) & 1);
-            for (int i = max(0, v_asked - TT_STAGES); i < v_asked; ++i) mbar_wait(&v_full[i % TT_STAGES], (i / TT_STAGES) & 1);
+            for (uint32_t i = ck > TT_STAGES ? ck - TT_STAGES : 0; i < ck; ++i) mbar_wait(&k_full[i % TT_STAGES], (i / TT_STAGES) & 1);
+            for (uint32_t i = cv > TT_STAGES ? cv - TT_STAGES : 0; i < cv; ++i) mbar_wait(&v_full[i % TT_STAGES], (i / TT_STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_qk = pt_idesc(LUMEN_PAGE, 0);
-            const uint32_t idesc_pv = pt_idesc(vw, 1);
-            const int k_steps = kw / 16;
-            auto issue_qk = [&](int c) {        // S[c & 1] = Q K(c)^T
-                const int st = c % TT_STAGES;
-                const uint32_t kt = smem_u32(sKV + st * STAGE_BYTES);
-#pragma unroll(D ? D / 16 : 1)
-                for (int ks = 0; ks < k_steps; ++ks) {
-                    const uint32_t aoff = (ks >> 2) * (PT_ROWS * 128) + (ks & 3) * 32;
-                    const uint32_t boff = (ks >> 2) * (LUMEN_PAGE * 128) + (ks & 3) * 32;
-                    pt_mma(tmem_base + (c & 1) * LUMEN_PAGE, pt_desc(smem_u32(sQ) + aoff, 16),
-                           pt_desc(kt + boff, 16), idesc_qk, ks > 0 ? 1u : 0u);
-                }
-                pt_commit(&k_empty[st]);
-                pt_commit(&s_full[c & 1]);
-            };
-            auto have_k = [&](int c) {
-                if (!mbar_wait(&k_full[c % TT_STAGES], (c / TT_STAGES) & 1)) return false;
-                pt_fence_after();
-                return true;
-            };
-            bool ok = true;
-            int c = 0;
-            for (int k = 0; ok && !*abort_flag; ++k) {
-                const int slot = k & 1;
-                if (!(ok = mbar_wait(&u_full[slot], (k >> 1) & 1))) break;
-                const int npages = s_unit[slot * TT_UNIT_INTS];
-                if (npages == 0) break;
-                if (!(ok = mbar_wait(q_ready, k & 1) && have_k(c))) break;
-                issue_qk(c);
-                for (int it = 0; it < npages; ++it, ++c) {
-                    if (*abort_flag) { ok = false; break; }
-                    if (it + 1 < npages) {
-                        if (!(ok = have_k(c + 1))) break;
-                        issue_qk(c + 1);
-                    }
-                    const int st = c % TT_STAGES;
-                    if (!(ok = mbar_wait(&v_full[st], (c / TT_STAGES) & 1) && mbar_wait(&p_ready[c & 1], (c >> 1) & 1))) break;
+        // The whole warp runs through this, so that what a product is told is the same in all lanes and known to be (with one
+        // thread alone S takes 770 cycles to issue instead of 640, O 490 instead of 280); one elected lane issues.
+        constexpr uint32_t idesc_qk = pt_idesc(LUMEN_PAGE, 0);
+        const uint32_t idesc_pv = pt_idesc(vw, 1);
+        const int k_steps = kw / 16;
+        const uint32_t q_at = smem_u32(sQ), kv_at = smem_u32(sKV);
+        bool ok = true;
+        uint32_t cs = 0, cv = 0;                        // pages whose S, whose O product has been issued
+        for (int k = 0; ok; ++k) {
+            const int slot = k & 1;
+            if (!(ok = tt_warp_wait(&u_full[slot], (k >> 1) & 1))) break;
+            const uint32_t npages = __shfl_sync(0xffffffffu, s_unit[slot * TT_UNIT_INTS], 0), first = cv, end = cv + npages;
+            if (npages == 0) break;
+            if (!(ok = tt_warp_wait(q_ready, k & 1))) break;
+            uint32_t spin = 0;
+            while (cv < end) {
+                // S of the next page as soon as its keys are there (its buffer's last weights went into a product that was
+                // issued before), else O of this page: neither waits for what the other lacks
+                if (cs < end && cs < cv + 2 && tt_warp_test(&k_full[cs % TT_STAGES], (cs / TT_STAGES) & 1)) {
                     pt_fence_after();
-                    const uint32_t vt = smem_u32(sKV + st * STAGE_BYTES + K_BYTES);
-                    const uint32_t pt = tmem_base + (c & 1) * LUMEN_PAGE;       // P lies over the first 32 columns of its scores
+                    const uint32_t st = cs % TT_STAGES, kt = kv_at + st * STAGE_BYTES, to = tmem_base + (cs & 1) * LUMEN_PAGE;
+                    if (tt_elect()) {
+#pragma unroll(D ? D / 16 : 1)
+                        for (int ks = 0; ks < k_steps; ++ks) {
+                            const uint32_t aoff = (ks >> 2) * (PT_ROWS * 128) + (ks & 3) * 32;
+                            const uint32_t boff = (ks >> 2) * (LUMEN_PAGE * 128) + (ks & 3) * 32;
+                            pt_mma(to, pt_desc(q_at + aoff, 16), pt_desc(kt + boff, 16), idesc_qk, ks > 0 ? 1u : 0u);
+                        }
+                        pt_commit(&s_full[cs & 1]);
+                        pt_commit(&k_empty[st]);
+                    }
+                    __syncwarp();
+                    ++cs;
+                    spin = 0;
+                } else if (cv < cs && tt_warp_test(&p_ready[cv & 1], (cv >> 1) & 1) && tt_warp_test(&v_full[cv % TT_STAGES], (cv / TT_STAGES) & 1)) {
+                    pt_fence_after();
+                    const uint32_t st = cv % TT_STAGES, vt = kv_at + st * STAGE_BYTES + K_BYTES;
+                    const uint32_t pt = tmem_base + (cv & 1) * LUMEN_PAGE;       // P lies over the first 32 columns of its scores
+                    if (tt_elect()) {
 #pragma unroll
-                    for (int kk = 0; kk < LUMEN_PAGE / 16; ++kk)
-                        pt_mma_ts(tmem_base + O_COL, pt + kk * 8,
-                                  pt_desc(vt + kk * (16 * 128), LUMEN_PAGE * 128), idesc_pv, (it > 0 || kk > 0) ? 1u : 0u);
-                    pt_commit(&v_empty[st]);
-                    pt_commit(&pv_done[c & 1]);
+                        for (int kk = 0; kk < LUMEN_PAGE / 16; ++kk)
+                            pt_mma_ts(tmem_base + O_COL, pt + kk * 8,
+                                      pt_desc(vt + kk * (16 * 128), LUMEN_PAGE * 128), idesc_pv, (cv > first || kk > 0) ? 1u : 0u);
+                        pt_commit(&v_empty[st]);
+                        pt_commit(&pv_done[cv & 1]);
+                    }
+                    __syncwarp();
+                    ++cv;
+                    spin = 0;
+                } else if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) {
+                    ok = false;
+                    break;
                 }
-                if (ok) pt_mbar_arrive(&u_empty[slot]);
             }
-            if (!ok) { *abort_flag = 1; atomicExch(t.err, 1); }
+            if (ok && lane == 0) pt_mbar_arrive(&u_empty[slot]);
         }
+        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(t.err, 1); }
     } else {
         const int r = (warp & 3) * 32 + lane;            // this thread's row of a unit
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
@@ -280,14 +306,11 @@ attn_tree_tc_kernel(const TreeTc t) {
         auto meet = [&]() {                              // all four warps
             __syncwarp();
             if (lane == 0) pt_mbar_arrive(together);
-            const bool w = mbar_wait(together, meetings & 1);
-            ++meetings;
-            return (bool)__all_sync(0xffffffffu, w);
+            return tt_warp_wait(together, meetings++ & 1);
         };
         TreeUnit x;
         auto read_unit = [&](int k) {
-            const bool w = mbar_wait(&u_full[k & 1], (k >> 1) & 1);
-            if (!__all_sync(0xffffffffu, w)) return false;
+            if (!tt_warp_wait(&u_full[k & 1], (k >> 1) & 1)) return false;
             volatile int* from = s_unit + (k & 1) * TT_UNIT_INTS;
             x.npages = from[0]; x.pg0 = from[1]; x.b = from[2]; x.n0 = from[3]; x.q = from[4]; x.start = from[5]; x.end = from[6];
             x.f0 = from[7]; x.kvh = from[8]; x.seg = from[9]; x.nseg = from[10];
@@ -333,17 +356,13 @@ attn_tree_tc_kernel(const TreeTc t) {
                 for (int i = lane; i < PT_ROWS; i += 32)
                     if (i < nrows) top = max(top, a.tok_pos[sq.n0 + (x.f0 + i) / G]);
                 lo_last = max(0, __reduce_max_sync(0xffffffffu, top) - a.window + 1);
-                if (!(ok = meet())) break;               // the last unit's positions are not needed any more
-                for (int i = threadIdx.x - 64; i < min(sq.q, TREE_MAX_NODES); i += 128) s_pos[i] = a.tok_pos[sq.n0 + i];
-                if (!(ok = meet())) break;
             }
             auto masked = [&](int jb) { return jb + LUMEN_PAGE > sq.start || jb < lo_last; };      // the same for every row
             bool any_masked = false;
             float m_ref = -INFINITY, l = 0.0f;
             for (int it = 0; it < npages; ++it, ++c) {
                 if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-                bool w = mbar_wait(&s_full[c & 1], (c >> 1) & 1);
-                if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+                if (!tt_warp_wait(&s_full[c & 1], (c >> 1) & 1)) { ok = false; break; }
                 pt_fence_after();
                 float s[64];
                 pt_ld64(lane_addr + (c & 1) * LUMEN_PAGE, s);
@@ -354,7 +373,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                 const int jb = (pg0 + it) * LUMEN_PAGE;
                 if (masked(jb)) {
                     any_masked = true;
-                    const unsigned long long seen = row_ok ? tree_seen(jb, sq, mask, a.W, prow, a.window, s_pos) : 0ull;
+                    const unsigned long long seen = row_ok ? tree_seen(jb, sq, mask, a.W, prow, a.window, a.tok_pos + sq.n0) : 0ull;
                     const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
@@ -363,8 +382,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                     }
                     // this thread's half of a value row, in every block of 64 numbers
                     const int st = c % TT_STAGES, vr = (threadIdx.x - 64) >> 1, half = threadIdx.x & 1;
-                    w = mbar_wait(&v_full[st], (c / TT_STAGES) & 1);
-                    if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+                    if (!tt_warp_wait(&v_full[st], (c / TT_STAGES) & 1)) { ok = false; break; }
                     unsigned char* row = sKV + st * STAGE_BYTES + K_BYTES + vr * 128 + half * 64;
                     bool bad = false;
                     for (int blk = 0; blk < vw >> 6; ++blk) {
@@ -426,8 +444,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                 l = l * corr + (l_even + l_odd);
                 // O is rescaled rarely; only then must the PV product of the page before be done
                 if (it > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
-                    w = mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1);
-                    if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+                    if (!tt_warp_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1)) { ok = false; break; }
                     pt_fence_after();
 #pragma unroll 1
                     for (int c0 = 0; c0 < vw; c0 += 32) {
@@ -452,8 +469,7 @@ attn_tree_tc_kernel(const TreeTc t) {
             const TreeUnit now = x;
             if (!(ok = read_unit(k + 1))) break;
             if (x.npages > 0) gather_q();
-            bool w = mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1);
-            if (!(ok = __all_sync(0xffffffffu, w))) break;
+            if (!(ok = tt_warp_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1))) break;
             pt_fence_after();
             if (any_masked && !(ok = meet())) break;         // every warp's s_bad
             const bool whole = now.nseg == 1, any_bad = any_masked && *(volatile int*)(s_bad + (k & 1)) == k + 1;
@@ -483,7 +499,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                     for (int it = 0; it < npages; ++it) {
                         const int jb = (pg0 + it) * LUMEN_PAGE;
                         if (!masked(jb)) continue;
-                        unsigned long long seen = tree_seen(jb, sq, mask, a.W, prow, a.window, s_pos);
+                        unsigned long long seen = tree_seen(jb, sq, mask, a.W, prow, a.window, a.tok_pos + sq.n0);
                         const int page = a.block_table[(size_t)now.b * a.bt_stride + pg0 + it];
                         const __nv_bfloat16* vt = vcache + ((size_t)((unsigned)page < (unsigned)a.n_pages ? page : 0) * a.nkv + now.kvh) *
                                                                (size_t)(LUMEN_PAGE * vw);
@@ -534,7 +550,7 @@ attn_tree_tc_kernel(const TreeTc t) {
 template <int D, bool CAP>
 static cudaError_t tt_go(const TreeTc& t, int max_segs, cudaStream_t stream) {
     const TreeArgs& a = t.a;
-    int smem = PT_ROWS * a.d * 2 + TT_STAGES * LUMEN_PAGE * (a.d + a.dv) * 2 + 384 + 4 * TREE_MAX_NODES;
+    int smem = PT_ROWS * a.d * 2 + TT_STAGES * LUMEN_PAGE * (a.d + a.dv) * 2 + 384;
     if (a.dv > 128 && smem < 116 * 1024) smem = 116 * 1024;      // such a block has the SM's tensor memory to itself
     auto k = attn_tree_tc_kernel<D, CAP>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -108,7 +108,7 @@ __device__ __forceinline__ unsigned long long tree_seen(int jb, const TreeSeq& s
         }
         const int left = s.end - jb;                      // no key beyond the sequence's end
         if (left < 64) own &= left > 0 ? (1ull << left) - 1 : 0;
-        if (window > 0) {
+        if (window > 0 && p - s.start >= window) {        // else no node is that far before it
             unsigned long long todo = own;
             while (todo) {
                 const int t = __ffsll((long long)todo) - 1;
