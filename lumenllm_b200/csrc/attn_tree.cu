@@ -272,8 +272,7 @@ __device__ __forceinline__ unsigned ta_pack(float lo, float hi) {
 }
 
 // Joins the segments of the sequences that have more than one, in rising order: a thread has four columns of a (token, head).
-// BASE2: the partial maxima are in units of log 2 (the tensor-core kernel's).
-template <typename T, bool BASE2>
+template <typename T>
 __global__ void __launch_bounds__(128)
 attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
     pdl_wait();
@@ -319,19 +318,19 @@ attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
         float mn = top;
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) mn = fmaxf(mn, x[i].x);
-        const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : BASE2 ? exp2f(top - mn) : expf(top - mn);
+        const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : expf(top - mn);
         o.x *= c; o.y *= c; o.z *= c; o.w *= c;
         l *= c;
         top = mn;
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;      // no key of that segment is in the row's sight
-            const float f = x[i].x == -INFINITY ? 1.0f : BASE2 ? exp2f(x[i].x - mn) : expf(x[i].x - mn);
+            const float f = x[i].x == -INFINITY ? 1.0f : expf(x[i].x - mn);
             o.x = fmaf(f, v[i].x, o.x); o.y = fmaf(f, v[i].y, o.y); o.z = fmaf(f, v[i].z, o.z); o.w = fmaf(f, v[i].w, o.w);
             l = fmaf(f, x[i].y, l);
         }
     }
-    const float inv = ta_close(BASE2 ? top * 0.6931471805599453f : top, l, a.sink, head);
+    const float inv = ta_close(top, l, a.sink, head);
     T* dst = (T*)a.out + ((size_t)n * a.nq + head) * a.dv + e;
     const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     if (quad_out && sizeof(T) == 2) {
@@ -343,22 +342,17 @@ attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
         if (e + i < a.dv) dst[i] = from_f32<T>(v[i]);
 }
 
-template <typename T>
-static cudaError_t ta_join(const TreeArgs& a, const int* tok_seq, int base2, cudaStream_t stream) {
-    const dim3 grid(a.N, ((a.dv + 3) / 4 * a.nq + 127) / 128);
-    return base2 ? lumen_launch(attn_tree_join_kernel<T, true>, grid, dim3(128), 0, stream, a, tok_seq)
-                 : lumen_launch(attn_tree_join_kernel<T, false>, grid, dim3(128), 0, stream, a, tok_seq);
-}
-
 template <typename T, int NC>
-static cudaError_t ta_go(const TreeArgs& a, int max_segs, cudaStream_t stream) {
+static cudaError_t ta_go(const TreeArgs& a, const int* tok_seq, int max_segs, cudaStream_t stream) {
     const int ks = ((a.d + 3) & ~3) + 4, wide = ks > 128 * NC ? ks : 128 * NC;
     const int smem = (TA_ROWS * ks + LUMEN_PAGE * wide + LUMEN_PAGE * TA_PROW) * (int)sizeof(float);
     auto k = attn_tree_kernel<T, NC>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)a.N * (a.nq / a.nkv) / TA_ROWS + a.B;
-    return lumen_launch(k, dim3((unsigned)(tiles * a.nkv), max_segs), dim3(TA_THREADS), smem, stream, a);
+    e = lumen_launch(k, dim3((unsigned)(tiles * a.nkv), max_segs), dim3(TA_THREADS), smem, stream, a);
+    if (e != cudaSuccess || max_segs == 1) return e;
+    return lumen_launch(attn_tree_join_kernel<T>, dim3(a.N, ((a.dv + 3) / 4 * a.nq + 127) / 128), dim3(128), 0, stream, a, tok_seq);
 }
 
 #include "attn_tree_tc.cuh"
@@ -369,12 +363,25 @@ static int ta_segs(int width) {
     return n < TREE_MAX_SEGS ? n : TREE_MAX_SEGS;
 }
 
+// Which kernel a call takes: 1 the tensor cores'.
+LUMEN_API int lumen_attn_tree_tc(const void* q, const void* kcache, const void* vcache, const void* out, int is_bf16, int d, int dv,
+                                 int layout, int v_layout, float scale) {
+    return tt_takes(is_bf16, d, dv, layout, v_layout, scale) && tt_aligned(q, kcache, vcache, out) ? 1 : 0;
+}
+// Thousands (1,024s) of float32 numbers of scratch that a call needs, -1: more than there can be.
+LUMEN_API int lumen_attn_tree_scratch(int tc, int B, int N, int width, int nq, int nkv, int d, int dv) {
+    if (B <= 0 || N <= 0 || width < 1 || nkv < 1 || nq < nkv || d < 1 || dv < 1) return 0;
+    const int G = nq / nkv;
+    const long long n = tc ? tt_floats(tt_blocks(B, N, width, nq, nkv, d, dv), dv)
+                           : ta_segs(width) == 1 ? 0 : (((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2) * nq * (dv + 2);
+    return n > 1024LL * 2147483647LL ? -1 : (int)((n + 1023) / 1024);
+}
+
 // q [N, nq, d], out [N, nq, dv] in the cache's type; keys [n_pages, nkv, 64, d], values [n_pages, nkv, 64, dv]; mask
-// [N, W] 64-bit words. Where width is above TREE_MIN_SEG sequences may be cut: parts then is float32 [pairs, nq, 2 + dv] for
-// pairs >= B tree_part_room(width, nq / nkv) + N, an even number.
+// [N, W] 64-bit words; tc and scratch (on 32 bytes) as the two functions above say.
 LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vcache, const int* block_table, int bt_stride,
                               int width, const int* cu_q, const int* seq_start, const int* tok_seq, const int* tok_pos,
-                              const void* mask, int W, void* out, float* parts, long long pairs, int is_bf16, int B, int N,
+                              const void* mask, int W, void* out, int tc, float* scratch, int scratch_k, int is_bf16, int B, int N,
                               int n_pages, int nq, int nkv, int d, int dv, int window, float scale, float softcap,
                               const float* sink, int layout, int v_layout, int* err, cudaStream_t stream) {
     if (B <= 0 || N <= 0) return 0;
@@ -384,23 +391,24 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     if ((layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || d % 64)) || (v_layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || dv % 64)))
         return LUMEN_ERR_UNSUPPORTED;
     const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = ta_segs(width);
-    if (((long long)N * G / TA_ROWS + B) * nkv * max_segs > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
-    if (max_segs > 1 && (!parts || (pairs & 1) || pairs < (long long)B * tree_part_room(width, G) + N)) return LUMEN_ERR_BAD_ARGUMENT;
-    float* part_o = parts ? parts + pairs * nq * 2 : nullptr;        // 16-byte rows where dv is a multiple of 4
+    if (((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
+    const int need = lumen_attn_tree_scratch(tc, B, N, width, nq, nkv, d, dv);
+    if (need < 0) return LUMEN_ERR_UNSUPPORTED;
+    if ((tc && (!tt_takes(is_bf16, d, dv, layout, v_layout, scale) || !tt_aligned(q, kcache, vcache, out))) || scratch_k < need ||
+        (need && !scratch) || ((uintptr_t)scratch & 31))
+        return LUMEN_ERR_BAD_ARGUMENT;
     const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0);
-    const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out, part_o,
-                        (float2*)parts, sink, bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec,
-                        scale, softcap};
-    const bool tc = tt_takes(a, is_bf16);
+    // the maxima and sums first: the rows behind them lie on 16 bytes where dv is a multiple of 4
+    const long long pairs = ((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2;
+    const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out,
+                        scratch ? scratch + pairs * nq * 2 : nullptr, (float2*)scratch, sink, bt_stride, width, W, B, N, n_pages, nq, nkv,
+                        d, dv, window, layout, v_layout, vec, scale, softcap};
     cudaError_t e;
-#define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, max_segs, stream) : ta_go<T, 4>(a, max_segs, stream))
-    e = tc ? tt_launch(a, max_segs, err, stream) : is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
+#define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, tok_seq, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, tok_seq, max_segs, stream) \
+                                                                                   : ta_go<T, 4>(a, tok_seq, max_segs, stream))
+    e = tc ? tt_launch(a, scratch, err, stream) : is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
 #undef TA_GO
     if (e != cudaSuccess) return (int)e;
-    if (max_segs > 1) {
-        e = is_bf16 ? ta_join<__nv_bfloat16>(a, tok_seq, tc, stream) : ta_join<float>(a, tok_seq, 0, stream);
-        if (e != cudaSuccess) return (int)e;
-    }
     LUMEN_LAUNCH_CHECK();
     return 0;
 }

@@ -1,12 +1,18 @@
 // Tree attention on the 5th-generation tensor cores: bfloat16, swizzled pages, keys and values of multiples of 64 up to 256.
 //
-// A unit of work is 128 rows (node, query head) of one kv head and one segment of the keys. It is walked a page at a time as
+// The work is blocks of 128 rows (node, query head) of one kv head, each with its pages. All of it, counted in pages, is dealt out
+// evenly over as many blocks of threads as fit the device: a piece, one block's part of a row block, is a unit. Row blocks
+// that one block has whole are finished there; of the others every piece leaves its unnormalised O, maximum and sum, which
+// a second kernel joins in rising order of the pages. So where a sequence is cut depends on the whole step, and its last bits with
+// it; the same step gives the same bits. (Cutting every sequence by its own length alone left the last of 1.3 rounds of equal
+// units to a third of the blocks: 64 nodes for 8 sequences after 4,000 to 6,000 tokens took 82 us.)
+//
+// A unit is walked a page at a time as
 // the prompts' kernel does: S = Q K^T into tensor memory (two buffers), the softmax by four warps with a row a thread, P as
 // bfloat16 over the scores it came from, O += P V in tensor memory; K and V tiles by bulk copies through two rings of two
-// stages. A block needs half of an SM, so that one's softmax runs under the other's products, and stays: as many blocks as fit the
-// device take the units in turn, so that no block is launched for a segment that a short sequence has not, and the next
-// unit's keys are under way while the last one's rows are written. Warp 0 finds the units, tells the others through
-// shared memory and asks for the tiles, warp 1 issues the products, warps 2 to 5 are the softmax and gather Q. Pages that hold
+// stages. A block needs half of an SM, so that one's softmax runs under the other's products. Warp 0 finds the units, tells the
+// others through shared memory and asks for the tiles, warp 1 issues the products, each fetches half of Q (while the last unit's
+// rows are written), warps 2 to 5 are the softmax. Pages that hold
 // nodes, or that a window cuts for some row, are masked: a row has one 64-bit word a page with the keys it sees.
 //
 // Weights are rounded to bfloat16 because the product takes both operands in one type: half a step, 2^-8 of a weight, which
@@ -23,19 +29,80 @@
 #define TT_THREADS 192
 #define TT_STAGES 2
 #define TT_RESCALE 8.0f
+#define TT_BAR_WORDS 48           // 8-byte words of barriers, units and flags
+#define TT_COST 3                 // what a row block costs beside its pages, in pages
+#define TT_SHARE 8                // a block's least share of the work, in pages
 
+// A place in the step's work: page `page` (counted from the first that the sequence's nodes see) of row block rb of sequence b.
+// b = B: the end.
+struct TreeCut {
+    int b, rb, page, unused;
+};
 struct TreeTc {
     TreeArgs a;
     float scale_log2;             // with CAP softcap * log2(e), what the tanh is multiplied by
     float cap_pre;                // with CAP scale / softcap
+    TreeCut* cuts;                // [blocks] where their work begins
     int* err;
 };
-
-// A unit: rows f0 .. f0 + 127 of sequence b and kv head kvh over pages pg0 .. pg0 + npages - 1 (npages 0: there is no more).
+// A unit: rows f0 .. f0 + 127 of sequence b and kv head kvh over pages pg0 .. pg0 + npages - 1 (npages 0: there is no more). slot: where
+// its partial result goes (0: it begins inside the row block, 1: it only ends inside), -1 for a whole row block.
 struct TreeUnit {
-    int npages, pg0, b, n0, q, start, end, f0, kvh, seg, nseg;
+    int npages, pg0, b, n0, q, start, end, f0, kvh, slot;
 };
-#define TT_UNIT_INTS 11
+#define TT_UNIT_INTS 10
+
+// A sequence's work: its row blocks (kv heads times tiles of 128 rows), the pages of each, and both together in pages.
+struct TreeWork {
+    int pg_lo, np, tiles;
+    long long all;
+};
+__device__ __forceinline__ TreeWork tt_work(const TreeArgs& a, const TreeSeq& s, int G) {
+    TreeWork w = {0, 0, 0, 0};
+    if (s.q > 0) {
+        tree_pages(s, a.window, w.pg_lo, w.np);
+        w.tiles = (int)(((long long)s.q * G + PT_ROWS - 1) / PT_ROWS);
+        w.all = (long long)w.tiles * a.nkv * (w.np + TT_COST);
+    }
+    return w;
+}
+// Where x pages of the work lie behind, found by a whole warp: run[i] is the work before thread i's `each` sequences. A cut is not made
+// within two pages of a row block's ends.
+__device__ __forceinline__ TreeCut tt_cut(const TreeArgs& a, int G, const long long* run, int each, long long x, int lane) {
+    TreeCut cut = {a.B, 0, 0, 0};
+    if (x >= run[TT_THREADS]) return cut;
+    int j = 0;
+    for (int i = 0; i < TT_THREADS; i += 32) {
+        const unsigned over = __ballot_sync(0xffffffffu, run[i + lane + 1] > x);
+        if (over) { j = i + __ffs(over) - 1; break; }
+    }
+    x -= run[j];
+    for (int b0 = j * each; b0 < (j + 1) * each; b0 += 32) {
+        const int b = b0 + lane;
+        TreeWork w = {0, 0, 0, 0};
+        if (b < min(a.B, (j + 1) * each)) w = tt_work(a, tree_seq(a.cu_q, a.seq_start, b, a.N, a.width), G);
+        long long sum = w.all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, x < sum);
+        if (!hit) {
+            x -= __shfl_sync(0xffffffffu, sum, 31);
+            continue;
+        }
+        const int src = __ffs(hit) - 1, np = __shfl_sync(0xffffffffu, w.np, src);
+        const long long off = x - __shfl_sync(0xffffffffu, sum - w.all, src);
+        cut.b = b0 + src;
+        cut.rb = (int)(off / (np + TT_COST));
+        cut.page = max(0, (int)(off - (long long)cut.rb * (np + TT_COST)) - TT_COST);
+        if (cut.page < 2) cut.page = 0;
+        else if (np - cut.page < 2) { ++cut.rb; cut.page = 0; }
+        break;
+    }
+    return cut;
+}
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
@@ -59,60 +126,12 @@ __device__ __forceinline__ bool tt_elect() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p)::"memory");
     return p != 0;
 }
-
-// The units in order, found by a whole warp: lane i holds sequence b0 + i. Sequences in order; of one, segments, then kv
-// heads, then row tiles, so that tiles which read the same keys run side by side.
-struct TreeFinder {
-    int b0, base, count, sum, tiles;
-    TreeSeq sq;
-    TreePlan plan;
-    __device__ __forceinline__ void chunk(const TreeArgs& a, int G, int lane) {
-        const int b = b0 + lane;
-        count = tiles = 0;
-        sq = TreeSeq{0, 0, 0, 0};
-        plan = TreePlan{0, 0, 1, 0, 0};
-        if (b < a.B) {
-            sq = tree_seq(a.cu_q, a.seq_start, b, a.N, a.width);
-            if (sq.q > 0) {
-                plan = tree_plan(sq, a.window, G);
-                tiles = (int)(((long long)sq.q * G + PT_ROWS - 1) / PT_ROWS);
-                count = tiles * plan.nseg * a.nkv;
-            }
-        }
-        sum = count;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-    }
-    __device__ __forceinline__ TreeUnit at(const TreeArgs& a, int G, int lane, int u) {
-        TreeUnit t = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        for (;;) {
-            const int total = __shfl_sync(0xffffffffu, sum, 31);
-            if (u < base + total) break;
-            base += total;
-            b0 += 32;
-            if (b0 >= a.B) return t;
-            chunk(a, G, lane);
-        }
-        const int src = __ffs(__ballot_sync(0xffffffffu, u < base + sum)) - 1;
-        const int x = u - base - __shfl_sync(0xffffffffu, sum - count, src), nt = __shfl_sync(0xffffffffu, tiles, src);
-        const int per = __shfl_sync(0xffffffffu, plan.per, src), rem = __shfl_sync(0xffffffffu, plan.rem, src);
-        t.b = b0 + src;
-        t.n0 = __shfl_sync(0xffffffffu, sq.n0, src);
-        t.q = __shfl_sync(0xffffffffu, sq.q, src);
-        t.start = __shfl_sync(0xffffffffu, sq.start, src);
-        t.end = __shfl_sync(0xffffffffu, sq.end, src);
-        t.nseg = __shfl_sync(0xffffffffu, plan.nseg, src);
-        t.f0 = (x % nt) * PT_ROWS;
-        t.kvh = (x / nt) % a.nkv;
-        t.seg = x / nt / a.nkv;
-        t.pg0 = __shfl_sync(0xffffffffu, plan.pg_lo, src) + t.seg * per + min(t.seg, rem);
-        t.npages = per + (t.seg < rem ? 1 : 0);
-        return t;
-    }
-};
+// 32 bytes in one instruction; to has to lie on 32 bytes.
+__device__ __forceinline__ void tt_store32(void* to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 
 // D: keys and values are D wide (64, 128), or (0) d and dv wide.
 template <int D, bool CAP>
@@ -146,8 +165,10 @@ attn_tree_tc_kernel(const TreeTc t) {
     uint64_t* together = q_ready + 1;          // the softmax warps wait for one another
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(together + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* s_bad = reinterpret_cast<int*>(tmem_slot + 2);        // [2] unit number + 1 where a visible place of a masked page holds no number
+    int* s_bad = reinterpret_cast<int*>(tmem_slot + 2);        // [2] unit number + 1 where a masked page holds a value that is no number
     volatile int* s_unit = s_bad + 2;          // [2][TT_UNIT_INTS]
+    TreeCut* s_cut = reinterpret_cast<TreeCut*>(s_bad + 2 + 2 * TT_UNIT_INTS);      // [2] where this block's work begins and ends
+    long long* s_run = reinterpret_cast<long long*>(bars + TT_BAR_WORDS);           // [TT_THREADS + 1]
 
     const int G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -159,7 +180,7 @@ attn_tree_tc_kernel(const TreeTc t) {
             mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1);
             mbar_init(&u_full[i], 1); mbar_init(&u_empty[i], 5);
         }
-        mbar_init(q_ready, 4);
+        mbar_init(q_ready, 2);
         mbar_init(together, 4);
         *abort_flag = 0;
         s_bad[0] = s_bad[1] = 0;
@@ -177,33 +198,126 @@ attn_tree_tc_kernel(const TreeTc t) {
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();      // nothing of this kernel touches global memory before this
     pdl_trigger();
+    // Every block adds up the step's work: a thread has `run` neighbouring sequences, the sums of whole threads are kept.
+    const int run = (a.B + TT_THREADS - 1) / TT_THREADS;
+    {
+        long long mine = 0;
+        for (int i = 0; i < run; ++i) {
+            const int b = threadIdx.x * run + i;
+            if (b < a.B) mine += tt_work(a, tree_seq(a.cu_q, a.seq_start, b, a.N, a.width), G).all;
+        }
+        long long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) s_run[TT_THREADS - warp] = sum;          // for a moment, the warps' sums at the end of the array
+        __syncthreads();
+        long long before = 0;
+        for (int w = 0; w < warp; ++w) before += s_run[TT_THREADS - w];
+        __syncthreads();
+        s_run[threadIdx.x + 1] = before + sum;
+        if (threadIdx.x == 0) s_run[0] = 0;
+        __syncthreads();
+    }
+    if (warp < 2) {
+        const long long total = s_run[TT_THREADS], share = max((total + gridDim.x - 1) / gridDim.x, (long long)TT_SHARE);
+        const TreeCut cut = tt_cut(a, G, s_run, run, (blockIdx.x + warp) * share, lane);
+        if (lane == 0) {
+            s_cut[warp] = cut;
+            if (warp == 0) t.cuts[blockIdx.x] = cut;
+        }
+    }
+    __syncthreads();
     const __nv_bfloat16* kcache = (const __nv_bfloat16*)a.kcache;
     const __nv_bfloat16* vcache = (const __nv_bfloat16*)a.vcache;
 
     // Counters of every role: k units and c pages since the block began; page c is in stage c % 2 of its ring and in
     // score buffer c & 1.
+    auto unit_at = [&](int slot) {
+        volatile int* from = s_unit + slot * TT_UNIT_INTS;
+        TreeUnit x;
+        x.npages = from[0]; x.pg0 = from[1]; x.b = from[2]; x.n0 = from[3]; x.q = from[4]; x.start = from[5]; x.end = from[6];
+        x.f0 = from[7]; x.kvh = from[8]; x.slot = from[9];
+        return x;
+    };
+    // Half of Q (by a whole warp) into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7). Rows that the sequence has not keep
+    // what was there: they are nobody's.
+    auto gather_q = [&](const TreeUnit& x, int half) {
+        const int nrows = min(PT_ROWS, x.q * G - x.f0), pieces = kw >> 3, rows = 32 / pieces, c = lane % pieces;
+        int row = half * (PT_ROWS / 2) + lane / pieces;
+        const int last = min(nrows, (half + 1) * (PT_ROWS / 2));
+        if (lane < rows * pieces) {
+            int tok = (x.f0 + row) / G, h = (x.f0 + row) - tok * G;
+            for (; row < last; row += rows) {
+                const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + ((size_t)(x.n0 + tok) * a.nq + x.kvh * G + h) * kw + 8 * c;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(sQ) + (c >> 3) * (PT_ROWS * 128) + row * 128 +
+                                                                               (((c & 7) ^ (row & 7)) << 4)), "l"(src)
+                             : "memory");
+                h += rows;
+                while (h >= G) { h -= G; ++tok; }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // Q is read by the tensor cores
+        __syncwarp();
+        if (lane == 0) pt_mbar_arrive(q_ready);
+    };
+
     if (warp == 0) {
-        TreeFinder find;
-        find.b0 = find.base = 0;
-        find.chunk(a, G, lane);
         uint32_t ck = 0, cv = 0;                        // K and V tiles asked for
         bool ok = true;
-        for (int k = 0, u = blockIdx.x; ok; ++k, u += gridDim.x) {
-            const TreeUnit x = find.at(a, G, lane, u);
+        TreeCut at = s_cut[0];
+        const TreeCut to = s_cut[1];
+        int b0 = at.b;                                  // lane i holds sequence b0 + i
+        TreeSeq sq_l;
+        TreeWork w_l;
+        auto hold = [&]() {
+            const int b = b0 + lane;
+            sq_l = b < a.B ? tree_seq(a.cu_q, a.seq_start, b, a.N, a.width) : TreeSeq{0, 0, 0, 0};
+            w_l = tt_work(a, sq_l, G);
+        };
+        hold();
+        for (int k = 0; ok; ++k) {
+            // the next piece of the block's work
+            TreeUnit x = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+            while (at.b < a.B) {
+                if (at.b >= b0 + 32) { b0 = at.b; hold(); }
+                const int src = at.b - b0, np = __shfl_sync(0xffffffffu, w_l.np, src), tiles = __shfl_sync(0xffffffffu, w_l.tiles, src);
+                if (at.rb >= tiles * a.nkv) { ++at.b; at.rb = at.page = 0; continue; }
+                const bool ends = at.b == to.b && at.rb == to.rb;
+                const int last = ends ? to.page : np;
+                if (at.b > to.b || (at.b == to.b && at.rb > to.rb) || (ends && at.page >= last)) break;
+                x.b = at.b;
+                x.n0 = __shfl_sync(0xffffffffu, sq_l.n0, src);
+                x.q = __shfl_sync(0xffffffffu, sq_l.q, src);
+                x.start = __shfl_sync(0xffffffffu, sq_l.start, src);
+                x.end = __shfl_sync(0xffffffffu, sq_l.end, src);
+                x.pg0 = __shfl_sync(0xffffffffu, w_l.pg_lo, src) + at.page;
+                x.npages = last - at.page;
+                x.kvh = at.rb / tiles;
+                x.f0 = (at.rb - x.kvh * tiles) * PT_ROWS;
+                x.slot = at.page > 0 ? 0 : last < np ? 1 : -1;
+                ++at.rb;
+                at.page = 0;
+                break;
+            }
             const int slot = k & 1;
             if (!(ok = tt_warp_wait(&u_empty[slot], ((k >> 1) & 1) ^ 1))) break;
             if (lane == 0) {
-                volatile int* to = s_unit + slot * TT_UNIT_INTS;
-                to[0] = x.npages; to[1] = x.pg0; to[2] = x.b; to[3] = x.n0; to[4] = x.q; to[5] = x.start; to[6] = x.end;
-                to[7] = x.f0; to[8] = x.kvh; to[9] = x.seg; to[10] = x.nseg;
+                volatile int* told = s_unit + slot * TT_UNIT_INTS;
+                told[0] = x.npages; told[1] = x.pg0; told[2] = x.b; told[3] = x.n0; told[4] = x.q; told[5] = x.start; told[6] = x.end;
+                told[7] = x.f0; told[8] = x.kvh; told[9] = x.slot;
                 pt_mbar_arrive(&u_full[slot]);
             }
             if (x.npages == 0) break;
             const int* bt = a.block_table + (size_t)x.b * a.bt_stride + x.pg0;
             const uint32_t first = cv, end = cv + x.npages;
+            bool q_here = false;
             int ids = 0, before = 0;                    // page numbers 32 at a time, and the ones before them
             uint32_t spin = 0;
-            while (cv < end) {
+            while (cv < end || !q_here) {
                 // whichever slot is free: K tiles run ahead of V tiles, their slots come free earlier
                 if (ck < end && tt_warp_test(&k_empty[ck % TT_STAGES], ((ck / TT_STAGES) & 1) ^ 1)) {
                     const uint32_t i = ck - first, st = ck % TT_STAGES;
@@ -231,6 +345,12 @@ attn_tree_tc_kernel(const TreeTc t) {
                     ++cv;
                     spin = 0;
                 }
+                // half of Q, when the S product of the page before this unit has given its slot back (it was the last to read Q)
+                if (!q_here && ck > first && tt_warp_test(&k_empty[(first + 1) % TT_STAGES], (((first + 1) / TT_STAGES) & 1) ^ 1)) {
+                    gather_q(x, 0);
+                    q_here = true;
+                    spin = 0;
+                }
                 if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
             }
         }
@@ -252,8 +372,12 @@ attn_tree_tc_kernel(const TreeTc t) {
         for (int k = 0; ok; ++k) {
             const int slot = k & 1;
             if (!(ok = tt_warp_wait(&u_full[slot], (k >> 1) & 1))) break;
-            const uint32_t npages = __shfl_sync(0xffffffffu, s_unit[slot * TT_UNIT_INTS], 0), first = cv, end = cv + npages;
-            if (npages == 0) break;
+            const TreeUnit x = unit_at(slot);
+            const uint32_t first = cv, end = cv + x.npages;
+            if (x.npages == 0) break;
+            // half of Q, once the last unit's S products have read theirs; the other half is warp 0's
+            if (cs > 0 && !(ok = tt_warp_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1))) break;
+            gather_q(x, 1);
             if (!(ok = tt_warp_wait(q_ready, k & 1))) break;
             uint32_t spin = 0;
             while (cv < end) {
@@ -301,7 +425,6 @@ attn_tree_tc_kernel(const TreeTc t) {
     } else {
         const int r = (warp & 3) * 32 + lane;            // this thread's row of a unit
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-        const __nv_bfloat16* q = (const __nv_bfloat16*)a.q;
         int meetings = 0;
         auto meet = [&]() {                              // all four warps
             __syncwarp();
@@ -313,36 +436,11 @@ attn_tree_tc_kernel(const TreeTc t) {
             if (!tt_warp_wait(&u_full[k & 1], (k >> 1) & 1)) return false;
             volatile int* from = s_unit + (k & 1) * TT_UNIT_INTS;
             x.npages = from[0]; x.pg0 = from[1]; x.b = from[2]; x.n0 = from[3]; x.q = from[4]; x.start = from[5]; x.end = from[6];
-            x.f0 = from[7]; x.kvh = from[8]; x.seg = from[9]; x.nseg = from[10];
+            x.f0 = from[7]; x.kvh = from[8]; x.slot = from[9];
             return true;
-        };
-        // Q: 128 rows into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7); rows beyond the sequence's are zeros.
-        // The products that read the last unit's Q are done: this warp has seen their last scores.
-        auto gather_q = [&]() {
-            const int nrows = min(PT_ROWS, x.q * G - x.f0), qpieces = kw >> 3;
-            constexpr int QL = 8;                        // loads a thread has under way
-            for (int base = threadIdx.x - 64; base < PT_ROWS * qpieces; base += QL * 128) {
-                uint4 v[QL];
-#pragma unroll
-                for (int i = 0; i < QL; ++i) {
-                    const int idx = base + i * 128, qr = idx / qpieces, c = idx - qr * qpieces, f = x.f0 + qr;
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (qr < nrows) v[i] = *reinterpret_cast<const uint4*>(q + ((size_t)(x.n0 + f / G) * a.nq + x.kvh * G + f % G) * kw + 8 * c);
-                }
-#pragma unroll
-                for (int i = 0; i < QL; ++i) {
-                    const int idx = base + i * 128, qr = idx / qpieces, c = idx - qr * qpieces;
-                    if (idx < PT_ROWS * qpieces)
-                        *reinterpret_cast<uint4*>(sQ + (c >> 3) * (PT_ROWS * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[i];
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // Q is read by the tensor cores
-            __syncwarp();
-            if (lane == 0) pt_mbar_arrive(q_ready);
         };
         int c = 0;
         bool ok = read_unit(0);
-        if (ok && x.npages > 0) gather_q();
         for (int k = 0; ok && x.npages > 0; ++k) {
             const TreeSeq sq = {x.n0, x.q, x.start, x.end};
             const int nrows = min(PT_ROWS, sq.q * G - x.f0), f = x.f0 + min(r, nrows - 1), node = f / G, head = x.kvh * G + f % G;
@@ -414,7 +512,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                     mx4[2] = pt_max3(mx4[2], s[j + 4], s[j + 5]);
                     mx4[3] = pt_max3(mx4[3], s[j + 6], s[j + 7]);
                 }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * t.scale_log2;
+                const float mx = row_ok ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * t.scale_log2 : -INFINITY;
                 // reference for the exponentials: moved only when the maximum has grown a lot
                 float corr = 1.0f;
                 if (mx > m_ref + TT_RESCALE || m_ref == -INFINITY) {
@@ -465,14 +563,10 @@ attn_tree_tc_kernel(const TreeTc t) {
                 if (lane == 0) pt_mbar_arrive(&p_ready[c & 1]);
             }
             if (!ok) break;
-            // the next unit's Q while the last product runs
-            const TreeUnit now = x;
-            if (!(ok = read_unit(k + 1))) break;
-            if (x.npages > 0) gather_q();
             if (!(ok = tt_warp_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1))) break;
             pt_fence_after();
             if (any_masked && !(ok = meet())) break;         // every warp's s_bad
-            const bool whole = now.nseg == 1, any_bad = any_masked && *(volatile int*)(s_bad + (k & 1)) == k + 1;
+            const bool whole = x.slot < 0, any_bad = any_masked && *(volatile int*)(s_bad + (k & 1)) == k + 1;
             float mul = 1.0f;
             __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((size_t)n * a.nq + head) * vw;
             float* part = nullptr;
@@ -485,7 +579,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                     mul = fr / (l * fr + exp2f(sk - top));
                 }
             } else {
-                const long long at = (tree_part_base(now.b, sq.n0, a.width, G) + (long long)node * now.nseg + now.seg) * a.nq + head;
+                const size_t at = (size_t)(2 * blockIdx.x + x.slot) * PT_ROWS + r;
                 part = a.part_o + at * vw;
                 if (row_ok) a.part_ml[at] = make_float2(m_ref, l);
             }
@@ -500,8 +594,8 @@ attn_tree_tc_kernel(const TreeTc t) {
                         const int jb = (pg0 + it) * LUMEN_PAGE;
                         if (!masked(jb)) continue;
                         unsigned long long seen = tree_seen(jb, sq, mask, a.W, prow, a.window, a.tok_pos + sq.n0);
-                        const int page = a.block_table[(size_t)now.b * a.bt_stride + pg0 + it];
-                        const __nv_bfloat16* vt = vcache + ((size_t)((unsigned)page < (unsigned)a.n_pages ? page : 0) * a.nkv + now.kvh) *
+                        const int page = a.block_table[(size_t)x.b * a.bt_stride + pg0 + it];
+                        const __nv_bfloat16* vt = vcache + ((size_t)((unsigned)page < (unsigned)a.n_pages ? page : 0) * a.nkv + x.kvh) *
                                                                (size_t)(LUMEN_PAGE * vw);
                         while (seen) {
                             const int key = __ffsll((long long)seen) - 1;
@@ -515,23 +609,26 @@ attn_tree_tc_kernel(const TreeTc t) {
                 }
                 if (row_ok && whole) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 v;
-                        v.x = pack_bf16(ov[j] * mul, ov[j + 1] * mul);
-                        v.y = pack_bf16(ov[j + 2] * mul, ov[j + 3] * mul);
-                        v.z = pack_bf16(ov[j + 4] * mul, ov[j + 5] * mul);
-                        v.w = pack_bf16(ov[j + 6] * mul, ov[j + 7] * mul);
-                        *reinterpret_cast<uint4*>(dst + c0 + j) = v;
+                    for (int j = 0; j < 32; j += 16) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = pack_bf16(ov[j + 2 * i] * mul, ov[j + 2 * i + 1] * mul);
+                        tt_store32(dst + c0 + j, w);
                     }
                 } else if (row_ok) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(part + c0 + j) = make_float4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
+                    for (int j = 0; j < 32; j += 8) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(ov[j + i]);
+                        tt_store32(part + c0 + j, w);
+                    }
                 }
             }
             pt_fence_before();                           // O has been read: the next unit's products may write it
             __syncwarp();
             if (lane == 0) pt_mbar_arrive(&u_empty[k & 1]);
+            if (!(ok = read_unit(k + 1))) break;
         }
         if (!ok) {
             *abort_flag = 1;
@@ -547,29 +644,111 @@ attn_tree_tc_kernel(const TreeTc t) {
     }
 }
 
-template <int D, bool CAP>
-static cudaError_t tt_go(const TreeTc& t, int max_segs, cudaStream_t stream) {
+// Joins the pieces of the row blocks that were cut. Blocks x = i - 1 have the cut where block i of the kernel before began its work: the
+// first cut of a row block joins all of its pieces, in the order of their pages; a thread has four columns of a row.
+__global__ void __launch_bounds__(256)
+attn_tree_tc_join_kernel(const TreeTc t, int blocks) {
+    pdl_wait();
+    pdl_trigger();
     const TreeArgs& a = t.a;
-    int smem = PT_ROWS * a.d * 2 + TT_STAGES * LUMEN_PAGE * (a.d + a.dv) * 2 + 384;
-    if (a.dv > 128 && smem < 116 * 1024) smem = 116 * 1024;      // such a block has the SM's tensor memory to itself
-    auto k = attn_tree_tc_kernel<D, CAP>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    // no more units than these come of the tokens and the page table, whatever the lengths are
-    const long long units = ((long long)a.N * (a.nq / a.nkv) / PT_ROWS + a.B) * a.nkv * max_segs;
-    const long long most = 148 * (smem <= 113 * 1024 ? 2 : 1);      // blocks that are resident at once
-    return lumen_launch(k, dim3((unsigned)(units < most ? units : most)), dim3(TT_THREADS), smem, stream, t);
+    const int i = blockIdx.x + 1, lane = threadIdx.x & 31;
+    const TreeCut cut = t.cuts[i], before = t.cuts[i - 1];
+    if (cut.page == 0 || (before.page > 0 && before.b == cut.b && before.rb == cut.rb)) return;
+    const int G = a.nq / a.nkv;
+    const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
+    const int tiles = tt_work(a, sq, G).tiles, kvh = cut.rb / tiles, f0 = (cut.rb - kvh * tiles) * PT_ROWS;
+    const int quads = a.dv >> 2, idx = blockIdx.y * 256 + threadIdx.x, row = idx / quads, e = (idx - row * quads) * 4;
+    int pieces = 2;                                     // block i - 1's and block i's, and of those that begin in this row block too
+    for (int j = i + 1; j < blocks; j += 32) {
+        TreeCut c = {-1, 0, 0, 0};
+        if (j + lane < blocks) c = t.cuts[j + lane];
+        const unsigned out = __ballot_sync(0xffffffffu, !(c.b == cut.b && c.rb == cut.rb && c.page > 0));
+        pieces += out ? __ffs(out) - 1 : 32;
+        if (out) break;
+    }
+    if (row >= min(PT_ROWS, sq.q * G - f0)) return;
+    constexpr int BATCH = 8;                            // pieces whose loads are under way together
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f, top = -INFINITY;
+    for (int s0 = 0; s0 < pieces; s0 += BATCH) {
+        float2 x[BATCH];
+        float4 v[BATCH];
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            x[s] = make_float2(-INFINITY, 0.0f);
+            v[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s0 + s < pieces) {
+                const size_t at = (size_t)(2 * (i - 1 + s0 + s) + (s0 + s == 0 ? 1 : 0)) * PT_ROWS + row;
+                x[s] = a.part_ml[at];
+                v[s] = *reinterpret_cast<const float4*>(a.part_o + at * a.dv + e);
+            }
+        }
+        float mn = top;
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) mn = fmaxf(mn, x[s].x);
+        // weights in units of log 2; without a maximum there is no weight, or a score that is no number
+        const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(top - mn);
+        o.x *= c; o.y *= c; o.z *= c; o.w *= c;
+        l *= c;
+        top = mn;
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            if (x[s].x == -INFINITY && x[s].y == 0.0f) continue;
+            const float f = x[s].x == -INFINITY ? 1.0f : exp2f(x[s].x - mn);
+            o.x = fmaf(f, v[s].x, o.x); o.y = fmaf(f, v[s].y, o.y); o.z = fmaf(f, v[s].z, o.z); o.w = fmaf(f, v[s].w, o.w);
+            l = fmaf(f, x[s].y, l);
+        }
+    }
+    const int f = f0 + row, head = kvh * G + f % G;
+    const float inv = ta_close(top * 0.6931471805599453f, l, a.sink, head);
+    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv + e) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
-// Whether the kernel takes these arguments: 16-byte aligned operands are what bulk copies and its vector loads need.
-static bool tt_takes(const TreeArgs& a, int is_bf16) {
-    return is_bf16 && a.layout == LUMEN_LAYOUT_SW128 && a.v_layout == LUMEN_LAYOUT_SW128 && a.d <= 256 && a.dv <= 256 && a.scale > 0.0f &&
-           !(((uintptr_t)a.q | (uintptr_t)a.kcache | (uintptr_t)a.vcache | (uintptr_t)a.out | (uintptr_t)a.part_o) & 15);
+// What a call's blocks need: shared memory, blocks that are resident at once (and no more than the work can come to, whatever the
+// lengths are), and float32 numbers of scratch: two partial results a block and the cuts.
+static int tt_smem(int d, int dv) {
+    const int smem = PT_ROWS * d * 2 + TT_STAGES * LUMEN_PAGE * (d + dv) * 2 + TT_BAR_WORDS * 8 + (TT_THREADS + 1) * 8;
+    return dv > 128 && smem < 116 * 1024 ? 116 * 1024 : smem;        // values beyond 128: all of the SM's tensor memory for one block
 }
-static cudaError_t tt_launch(const TreeArgs& a, int max_segs, int* err, cudaStream_t stream) {
+static int tt_blocks(int B, int N, int width, int nq, int nkv, int d, int dv) {
+    const long long most = 148 * (tt_smem(d, dv) <= 113 * 1024 ? 2 : 1);
+    const long long work = ((long long)N * (nq / nkv) / PT_ROWS + B) * nkv * ((long long)width + TT_COST);
+    const long long n = (work + TT_SHARE - 1) / TT_SHARE;
+    return (int)(n < most ? n : most);
+}
+static long long tt_floats(int blocks, int dv) { return (long long)blocks * (2 * PT_ROWS * (dv + 2) + 4); }
+
+template <int D, bool CAP>
+static cudaError_t tt_go(const TreeTc& t, int blocks, cudaStream_t stream) {
+    const TreeArgs& a = t.a;
+    const int smem = tt_smem(a.d, a.dv);
+    auto k = attn_tree_tc_kernel<D, CAP>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = lumen_launch(k, dim3(blocks), dim3(TT_THREADS), smem, stream, t);
+    if (e == cudaSuccess && blocks > 1)
+        e = lumen_launch(attn_tree_tc_join_kernel, dim3(blocks - 1, PT_ROWS * a.dv / 1024), dim3(256), 0, stream, t, blocks);
+    return e;
+}
+
+// Whether the kernel takes these arguments (beside the operands' places, which bulk copies and its wide stores need).
+static bool tt_takes(int is_bf16, int d, int dv, int layout, int v_layout, float scale) {
+    return is_bf16 && layout == LUMEN_LAYOUT_SW128 && v_layout == LUMEN_LAYOUT_SW128 && d <= 256 && dv <= 256 && scale > 0.0f;
+}
+static bool tt_aligned(const void* q, const void* kcache, const void* vcache, const void* out) {
+    return !(((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache) & 15) && !((uintptr_t)out & 31);
+}
+static cudaError_t tt_launch(TreeArgs a, float* scratch, int* err, cudaStream_t stream) {
+    const int blocks = tt_blocks(a.B, a.N, a.width, a.nq, a.nkv, a.d, a.dv);
+    const size_t rows = (size_t)blocks * 2 * PT_ROWS;
+    a.part_o = scratch;
+    a.part_ml = (float2*)(scratch + rows * a.dv);
     const bool cap = a.softcap > 0.0f;
-    const TreeTc t = {a, (cap ? a.softcap : a.scale) * 1.4426950408889634f, cap ? a.scale / a.softcap : 0.0f, err};
-    if (a.d == 128 && a.dv == 128) return cap ? tt_go<128, true>(t, max_segs, stream) : tt_go<128, false>(t, max_segs, stream);
-    if (a.d == 64 && a.dv == 64) return cap ? tt_go<64, true>(t, max_segs, stream) : tt_go<64, false>(t, max_segs, stream);
-    return cap ? tt_go<0, true>(t, max_segs, stream) : tt_go<0, false>(t, max_segs, stream);
+    const TreeTc t = {a, (cap ? a.softcap : a.scale) * 1.4426950408889634f, cap ? a.scale / a.softcap : 0.0f,
+                      (TreeCut*)(scratch + rows * (a.dv + 2)), err};
+#define TT_GO(D) (cap ? tt_go<D, true>(t, blocks, stream) : tt_go<D, false>(t, blocks, stream))
+    if (a.d == 128 && a.dv == 128) return TT_GO(128);
+    if (a.d == 64 && a.dv == 64) return TT_GO(64);
+    return TT_GO(0);
+#undef TT_GO
 }

@@ -25,10 +25,17 @@ __device__ __forceinline__ TreeSeq tree_seq(const int* cu_q, const int* seq_star
     return s;
 }
 
-// Pages [pg_lo, pg_lo + np) that some node sees, in nseg segments of per or per + 1 pages (the first rem have one more).
+// Pages [pg_lo, pg_lo + np) are those that some node of the sequence may see.
+__device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg_lo, int& np) {
+    // no node stands before the cached tokens' end
+    const int lo = window > 0 ? min(max(0, s.start - window + 1), s.end - 1) : 0;
+    pg_lo = lo / LUMEN_PAGE;
+    np = max((s.end - 1) / LUMEN_PAGE - pg_lo + 1, 1);
+}
+// The general kernel's cut of them: nseg segments of per or per + 1 pages (the first rem have one more).
 // A segment's partial result is rows x dv float32, its keys and values are pages x 64 x (d + dv) numbers: with a page for
-// eight rows at least, bfloat16 partials come to an eighth of what the segment reads. The cut depends on the sequence
-// alone, never on its neighbours in the batch or the page table's width.
+// eight rows at least, partials come to an eighth (bfloat16) or a sixteenth of what the segment reads. The cut depends on the
+// sequence alone, never on its neighbours in the batch or the page table's width.
 struct TreePlan {
     int pg_lo, np, nseg, per, rem;
     __device__ __forceinline__ int first(int seg) const { return pg_lo + seg * per + min(seg, rem); }
@@ -36,10 +43,7 @@ struct TreePlan {
 };
 __device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int G) {
     TreePlan p;
-    // no node stands before the cached tokens' end
-    const int lo = window > 0 ? min(max(0, s.start - window + 1), s.end - 1) : 0;
-    p.pg_lo = lo / LUMEN_PAGE;
-    p.np = max((s.end - 1) / LUMEN_PAGE - p.pg_lo + 1, 1);
+    tree_pages(s, window, p.pg_lo, p.np);
     const long long rows = (long long)s.q * G;
     const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 7) / 8));
     p.nseg = min((p.np + seg - 1) / seg, TREE_MAX_SEGS);

@@ -1956,7 +1956,6 @@ def attn_prefill(q, kcache, vcache, block_table, cu_q, seq_start, q_lens, window
 # ------------------------------------------------------------------ trees of drafted tokens
 
 TREE_MAX_NODES = 256      # nodes of a sequence that masks and walks cover: TREE_MAX_NODES of csrc/tree_plan.cuh
-TREE_MIN_SEG = 4          # pages of a page table that no sequence is cut in: TREE_MIN_SEG there
 
 StepTables = namedtuple("StepTables", "cu_q tok_seq cache_pos tok_pos slot_map block_table tree_mask")
 
@@ -2072,15 +2071,16 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
         return out
     sink = _sink_arg(sink, nq, q.device)
     width = block_table.shape[1]
-    # (token, segment) pairs of partial results: what csrc/tree_plan.cuh can come to, whatever the lengths are
-    pairs = (B * -(-8 * width // (nq // nkv)) + N + 1) // 2 * 2 if width > TREE_MIN_SEG else 0
-    parts = torch.empty((pairs * nq * (dv + 2),), dtype=F32, device=q.device) if pairs else None
+    bf16 = _is_bf16(q)
+    where = (ptr(q), ptr(kcache), ptr(vcache), ptr(out))
+    tc = int_fn("attn_tree", "lumen_attn_tree_tc", [P] * 4 + [c_int] * 5 + [c_float])(*where, bf16, d, dv, layout, v_layout, scale)
+    scratch_k = int_fn("attn_tree", "lumen_attn_tree_scratch", [c_int] * 8)(tc, B, N, width, nq, nkv, d, dv)
+    scratch = torch.empty((max(scratch_k, 0) * 1024,), dtype=F32, device=q.device) if scratch_k else None
     f = fn("attn_tree", "lumen_attn_tree",
-           [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, P, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-            c_int, c_float, c_float, P, c_int, c_int, P, P])
-    check(f(ptr(q), ptr(kcache), ptr(vcache), ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq),
-            ptr(tok_pos), ptr(tree_mask), words, ptr(out), ptr(parts), pairs, _is_bf16(q), B, N, n_pages, nq, nkv, d, dv, int(window),
-            float(scale), float(softcap), ptr(sink), int(layout), int(v_layout), ptr(error_flag(q.device)), stream_ptr()), "attn_tree")
+           [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, c_int, P] + [c_int] * 10 + [c_float, c_float, P, c_int, c_int, P, P])
+    check(f(*where[:3], ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq), ptr(tok_pos),
+            ptr(tree_mask), words, where[3], tc, ptr(scratch), scratch_k, bf16, B, N, n_pages, nq, nkv, d, dv, int(window), float(scale),
+            float(softcap), ptr(sink), int(layout), int(v_layout), ptr(error_flag(q.device)), stream_ptr()), "attn_tree")
     return out
 
 

@@ -159,18 +159,35 @@ def test_rows_behind_the_last_sequence_and_wider_tables_change_nothing():
         assert torch.equal(got[:27], want) and bool((got[27:] == 7.0).all())
 
 
-def test_a_sequence_is_the_same_alone_and_in_any_batch():
-    for dtype, d in ((BF16, 128), (BF16, 64), (F32, 64)):
+def test_the_same_step_gives_the_same_bits_and_the_general_kernel_in_any_batch():
+    """A step again: the same bits. A sequence alone: the same bits from the general kernel, whose cut of the keys is the
+    sequence's own, and within what arithmetic allows from the tensor cores', whose cut is the step's."""
+    for dtype, d in ((BF16, 128), (BF16, 64), (F32, 64), (BF16, 48)):
         c = D.Case([1500, 64, 0, 900], [16, 64, 3, 31], 8, 2, d, dtype=dtype, seed=8)
         whole = attend(c)
+        assert torch.equal(attend(c), whole)
+        ref, size = c.reference()
+        tol = c.bound(ref, size, rounded_weights=dtype == BF16)
         n0 = 0
         a = c.arrays()
         for b, n in enumerate(c.qlens):
             alone = attend(c, q=c.q[n0:n0 + n], block_table=a["block_table"][b:b + 1], cu_q=torch.tensor([0, n], dtype=I32),
                            seq_start=a["seq_start"][b:b + 1], tok_seq=torch.zeros(n, dtype=I32), tok_pos=a["tok_pos"][n0:n0 + n],
                            tree_mask=a["tree_mask"][n0:n0 + n])
-            assert torch.equal(alone, whole[n0:n0 + n])
+            if dtype == F32 or d == 48:
+                assert torch.equal(alone, whole[n0:n0 + n])
+            assert bool(((alone.double() - ref[n0:n0 + n]).abs() <= tol[n0:n0 + n]).all())
             n0 += n
+
+
+def test_work_dealt_out_over_the_blocks():
+    """Steps whose row blocks are cut by many blocks, by none, and by few: long beside empty sequences, more sequences than a
+    block has threads."""
+    for starts, nodes, nq, nkv, d in (([9000], [3], 2, 1, 64), ([5000, 0, 1, 3000], [1, 2, 200, 64], 4, 1, 128),
+                                      ([17 * i % 130 for i in range(400)], [i % 4 for i in range(400)], 2, 2, 64),
+                                      ([100] * 40, [60] * 40, 8, 8, 64), ([2500], [256], 16, 1, 256)):
+        c = D.Case(starts, nodes, nq, nkv, d, seed=len(starts) + d)
+        close(c, attend(c))
 
 
 def test_lengths_and_pages_that_cannot_be_are_held_inside_the_arrays():
@@ -185,11 +202,13 @@ def test_lengths_and_pages_that_cannot_be_are_held_inside_the_arrays():
         table[1] = torch.tensor([-5, 10 ** 9, c.n_pages, -(1 << 31)] + [1 << 30] * (c.width - 4), dtype=I32)
         start = a["seq_start"].clone()
         start[1] = 10 ** 9
-        got = attend(c, block_table=table, seq_start=start)
-        assert torch.equal(got[:7], want[:7]) and torch.equal(got[16:], want[16:])
+        ref, size = c.reference()
+        tol = c.bound(ref, size, rounded_weights=dtype == BF16)
+        right = lambda got: bool(((got.double() - ref).abs() <= tol)[[i for i in range(21) if not 7 <= i < 16]].all())
+        assert right(want)
+        assert right(attend(c, block_table=table, seq_start=start))
         start[1] = -(1 << 31)
-        got = attend(c, block_table=table, seq_start=start, cu_q=torch.tensor([0, 7, 16, 1 << 30], dtype=I32))
-        assert torch.equal(got[:7], want[:7]) and torch.equal(got[16:], want[16:])
+        assert right(attend(c, block_table=table, seq_start=start, cu_q=torch.tensor([0, 7, 16, 1 << 30], dtype=I32)))
 
 
 def test_long_caches_beyond_32_bits():
