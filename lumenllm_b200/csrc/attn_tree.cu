@@ -364,9 +364,9 @@ static int ta_segs(int width) {
 }
 
 // Which kernel a call takes: 1 the tensor cores'.
-LUMEN_API int lumen_attn_tree_tc(const void* q, const void* kcache, const void* vcache, const void* out, int is_bf16, int d, int dv,
-                                 int layout, int v_layout, float scale) {
-    return tt_takes(is_bf16, d, dv, layout, v_layout, scale) && tt_aligned(q, kcache, vcache, out) ? 1 : 0;
+LUMEN_API int lumen_attn_tree_tc(const void* q, const void* kcache, const void* vcache, const void* out, int is_bf16, int B, int N,
+                                 int width, int nq, int nkv, int d, int dv, int layout, int v_layout, float scale) {
+    return nkv > 0 && nq >= nkv && tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale) && tt_aligned(q, kcache, vcache, out) ? 1 : 0;
 }
 // Thousands (1,024s) of float32 numbers of scratch that a call needs, -1: more than there can be.
 LUMEN_API int lumen_attn_tree_scratch(int tc, int B, int N, int width, int nq, int nkv, int d, int dv) {
@@ -394,7 +394,7 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     if (((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
     const int need = lumen_attn_tree_scratch(tc, B, N, width, nq, nkv, d, dv);
     if (need < 0) return LUMEN_ERR_UNSUPPORTED;
-    if ((tc && (!tt_takes(is_bf16, d, dv, layout, v_layout, scale) || !tt_aligned(q, kcache, vcache, out))) || scratch_k < need ||
+    if ((tc && (!tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale) || !tt_aligned(q, kcache, vcache, out))) || scratch_k < need ||
         (need && !scratch) || ((uintptr_t)scratch & 31))
         return LUMEN_ERR_BAD_ARGUMENT;
     const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0);

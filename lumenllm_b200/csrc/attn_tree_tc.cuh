@@ -11,8 +11,8 @@
 // the prompts' kernel does: S = Q K^T into tensor memory (two buffers), the softmax by four warps with a row a thread, P as
 // bfloat16 over the scores it came from, O += P V in tensor memory; K and V tiles by bulk copies through two rings of two
 // stages. A block needs half of an SM, so that one's softmax runs under the other's products. Warp 0 finds the units, tells the
-// others through shared memory and asks for the tiles, warp 1 issues the products, each fetches half of Q (while the last unit's
-// rows are written), warps 2 to 5 are the softmax. Pages that hold
+// others through shared memory and asks for the tiles, warp 1 fetches Q (while the last unit's rows are written) and issues the
+// products, warps 2 to 5 are the softmax. Pages that hold
 // nodes, or that a window cuts for some row, are masked: a row has one 64-bit word a page with the keys it sees.
 //
 // Weights are rounded to bfloat16 because the product takes both operands in one type: half a step, 2^-8 of a weight, which
@@ -31,7 +31,7 @@
 #define TT_RESCALE 8.0f
 #define TT_BAR_WORDS 48           // 8-byte words of barriers, units and flags
 #define TT_COST 3                 // what a row block costs beside its pages, in pages
-#define TT_SHARE 8                // a block's least share of the work, in pages
+#define TT_SHARE 5                // a block's least share of the work, in pages
 
 // A place in the step's work: page `page` (counted from the first that the sequence's nodes see) of row block rb of sequence b.
 // b = B: the end.
@@ -54,54 +54,19 @@ struct TreeUnit {
 
 // A sequence's work: its row blocks (kv heads times tiles of 128 rows), the pages of each, and both together in pages.
 struct TreeWork {
-    int pg_lo, np, tiles;
-    long long all;
+    int pg_lo, np, tiles, all;
 };
 __device__ __forceinline__ TreeWork tt_work(const TreeArgs& a, const TreeSeq& s, int G) {
     TreeWork w = {0, 0, 0, 0};
     if (s.q > 0) {
         tree_pages(s, a.window, w.pg_lo, w.np);
-        w.tiles = (int)(((long long)s.q * G + PT_ROWS - 1) / PT_ROWS);
-        w.all = (long long)w.tiles * a.nkv * (w.np + TT_COST);
+        w.tiles = (s.q * G + PT_ROWS - 1) / PT_ROWS;
+        w.all = w.tiles * a.nkv * (w.np + TT_COST);
     }
     return w;
 }
-// Where x pages of the work lie behind, found by a whole warp: run[i] is the work before thread i's `each` sequences. A cut is not made
-// within two pages of a row block's ends.
-__device__ __forceinline__ TreeCut tt_cut(const TreeArgs& a, int G, const long long* run, int each, long long x, int lane) {
-    TreeCut cut = {a.B, 0, 0, 0};
-    if (x >= run[TT_THREADS]) return cut;
-    int j = 0;
-    for (int i = 0; i < TT_THREADS; i += 32) {
-        const unsigned over = __ballot_sync(0xffffffffu, run[i + lane + 1] > x);
-        if (over) { j = i + __ffs(over) - 1; break; }
-    }
-    x -= run[j];
-    for (int b0 = j * each; b0 < (j + 1) * each; b0 += 32) {
-        const int b = b0 + lane;
-        TreeWork w = {0, 0, 0, 0};
-        if (b < min(a.B, (j + 1) * each)) w = tt_work(a, tree_seq(a.cu_q, a.seq_start, b, a.N, a.width), G);
-        long long sum = w.all;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, x < sum);
-        if (!hit) {
-            x -= __shfl_sync(0xffffffffu, sum, 31);
-            continue;
-        }
-        const int src = __ffs(hit) - 1, np = __shfl_sync(0xffffffffu, w.np, src);
-        const long long off = x - __shfl_sync(0xffffffffu, sum - w.all, src);
-        cut.b = b0 + src;
-        cut.rb = (int)(off / (np + TT_COST));
-        cut.page = max(0, (int)(off - (long long)cut.rb * (np + TT_COST)) - TT_COST);
-        if (cut.page < 2) cut.page = 0;
-        else if (np - cut.page < 2) { ++cut.rb; cut.page = 0; }
-        break;
-    }
-    return cut;
+__device__ __forceinline__ TreeWork tt_work_of(const TreeArgs& a, int b, int G) {
+    return b < a.B ? tt_work(a, tree_seq(a.cu_q, a.seq_start, b, a.N, a.width), G) : TreeWork{0, 0, 0, 0};
 }
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -161,14 +126,14 @@ attn_tree_tc_kernel(const TreeTc t) {
     uint64_t* pv_done = p_ready + 2;           // [2] the PV product of that page has finished
     uint64_t* u_full = pv_done + 2;            // [2] a unit is told
     uint64_t* u_empty = u_full + 2;            // [2] it has been worked off
-    uint64_t* q_ready = u_empty + 2;           // Q of the next unit is in place
-    uint64_t* together = q_ready + 1;          // the softmax warps wait for one another
+    uint64_t* together = u_empty + 2;          // the softmax warps wait for one another
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(together + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_bad = reinterpret_cast<int*>(tmem_slot + 2);        // [2] unit number + 1 where a masked page holds a value that is no number
     volatile int* s_unit = s_bad + 2;          // [2][TT_UNIT_INTS]
     TreeCut* s_cut = reinterpret_cast<TreeCut*>(s_bad + 2 + 2 * TT_UNIT_INTS);      // [2] where this block's work begins and ends
-    long long* s_run = reinterpret_cast<long long*>(bars + TT_BAR_WORDS);           // [TT_THREADS + 1]
+    volatile int* s_sum = reinterpret_cast<volatile int*>(s_cut + 2);               // [warps]
+    volatile int* s_first = s_sum + TT_THREADS / 32;                                // [7] the first unit's sequence
 
     const int G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -180,7 +145,6 @@ attn_tree_tc_kernel(const TreeTc t) {
             mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1);
             mbar_init(&u_full[i], 1); mbar_init(&u_empty[i], 5);
         }
-        mbar_init(q_ready, 2);
         mbar_init(together, 4);
         *abort_flag = 0;
         s_bad[0] = s_bad[1] = 0;
@@ -198,35 +162,65 @@ attn_tree_tc_kernel(const TreeTc t) {
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();      // nothing of this kernel touches global memory before this
     pdl_trigger();
-    // Every block adds up the step's work: a thread has `run` neighbouring sequences, the sums of whole threads are kept.
+    // Every block adds up the step's work, a thread the work of `run` neighbouring sequences; the threads whose sequences hold the
+    // ends of the block's share find the places there. A cut is not made within two pages of a row block's ends.
     const int run = (a.B + TT_THREADS - 1) / TT_THREADS;
     {
-        long long mine = 0;
-        for (int i = 0; i < run; ++i) {
-            const int b = threadIdx.x * run + i;
-            if (b < a.B) mine += tt_work(a, tree_seq(a.cu_q, a.seq_start, b, a.N, a.width), G).all;
-        }
-        long long sum = mine;
+        TreeWork w = tt_work_of(a, threadIdx.x * run, G);
+        const TreeWork w0 = w;
+        int mine = w.all;
+        for (int i = 1; i < run; ++i) mine += tt_work_of(a, threadIdx.x * run + i, G).all;
+        int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += v;
         }
-        if (lane == 31) s_run[TT_THREADS - warp] = sum;          // for a moment, the warps' sums at the end of the array
+        if (lane == 31) s_sum[warp] = sum;
         __syncthreads();
-        long long before = 0;
-        for (int w = 0; w < warp; ++w) before += s_run[TT_THREADS - w];
-        __syncthreads();
-        s_run[threadIdx.x + 1] = before + sum;
-        if (threadIdx.x == 0) s_run[0] = 0;
-        __syncthreads();
-    }
-    if (warp < 2) {
-        const long long total = s_run[TT_THREADS], share = max((total + gridDim.x - 1) / gridDim.x, (long long)TT_SHARE);
-        const TreeCut cut = tt_cut(a, G, s_run, run, (blockIdx.x + warp) * share, lane);
-        if (lane == 0) {
-            s_cut[warp] = cut;
-            if (warp == 0) t.cuts[blockIdx.x] = cut;
+        int total = 0;
+        sum -= mine;
+#pragma unroll
+        for (int i = 0; i < TT_THREADS / 32; ++i) {
+            if (i == warp) sum += total;
+            total += s_sum[i];
+        }
+        const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, TT_SHARE);
+#pragma unroll 1
+        for (int end = 0; end < 2; ++end) {
+            int x = ((int)blockIdx.x + end) * share;
+            TreeCut cut = {a.B, 0, 0, 0};
+            if (x >= total ? threadIdx.x != 0 : x < sum || x >= sum + mine) continue;
+            if (x < total) {
+                x -= sum;
+                cut.b = threadIdx.x * run;
+                w = w0;
+                while (x >= w.all) {
+                    x -= w.all;
+                    w = tt_work_of(a, ++cut.b, G);
+                }
+                cut.rb = x / (w.np + TT_COST);
+                cut.page = max(0, x - cut.rb * (w.np + TT_COST) - TT_COST);
+                if (cut.page < 2) cut.page = 0;
+                else if (w.np - cut.page < 2) {
+                    cut.page = 0;
+                    if (++cut.rb == w.tiles * a.nkv) {
+                        cut.rb = 0;
+                        do w = tt_work_of(a, ++cut.b, G);
+                        while (cut.b < a.B && w.all == 0);
+                    }
+                }
+            }
+            s_cut[end] = cut;
+            if (end == 0) {
+                t.cuts[blockIdx.x] = cut;
+                // what warp 0 needs for the block's first keys
+                if (cut.b < a.B) {
+                    const TreeSeq s = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
+                    s_first[0] = s.n0; s_first[1] = s.q; s_first[2] = s.start; s_first[3] = s.end;
+                    s_first[4] = w.pg_lo; s_first[5] = w.np; s_first[6] = w.tiles;
+                }
+            }
         }
     }
     __syncthreads();
@@ -242,48 +236,25 @@ attn_tree_tc_kernel(const TreeTc t) {
         x.f0 = from[7]; x.kvh = from[8]; x.slot = from[9];
         return x;
     };
-    // Half of Q (by a whole warp) into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7). Rows that the sequence has not keep
-    // what was there: they are nobody's.
-    auto gather_q = [&](const TreeUnit& x, int half) {
-        const int nrows = min(PT_ROWS, x.q * G - x.f0), pieces = kw >> 3, rows = 32 / pieces, c = lane % pieces;
-        int row = half * (PT_ROWS / 2) + lane / pieces;
-        const int last = min(nrows, (half + 1) * (PT_ROWS / 2));
-        if (lane < rows * pieces) {
-            int tok = (x.f0 + row) / G, h = (x.f0 + row) - tok * G;
-            for (; row < last; row += rows) {
-                const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + ((size_t)(x.n0 + tok) * a.nq + x.kvh * G + h) * kw + 8 * c;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(sQ) + (c >> 3) * (PT_ROWS * 128) + row * 128 +
-                                                                               (((c & 7) ^ (row & 7)) << 4)), "l"(src)
-                             : "memory");
-                h += rows;
-                while (h >= G) { h -= G; ++tok; }
-            }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // Q is read by the tensor cores
-        __syncwarp();
-        if (lane == 0) pt_mbar_arrive(q_ready);
-    };
 
     if (warp == 0) {
         uint32_t ck = 0, cv = 0;                        // K and V tiles asked for
         bool ok = true;
         TreeCut at = s_cut[0];
         const TreeCut to = s_cut[1];
-        int b0 = at.b;                                  // lane i holds sequence b0 + i
-        TreeSeq sq_l;
-        TreeWork w_l;
-        auto hold = [&]() {
-            const int b = b0 + lane;
-            sq_l = b < a.B ? tree_seq(a.cu_q, a.seq_start, b, a.N, a.width) : TreeSeq{0, 0, 0, 0};
-            w_l = tt_work(a, sq_l, G);
-        };
-        hold();
+        int b0 = at.b, held = 1;                        // lane i holds sequence b0 + i, `held` of them; at first the one that is known
+        TreeSeq sq_l = {s_first[0], s_first[1], s_first[2], s_first[3]};
+        TreeWork w_l = {s_first[4], s_first[5], s_first[6], 0};
         for (int k = 0; ok; ++k) {
             // the next piece of the block's work
             TreeUnit x = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
             while (at.b < a.B) {
-                if (at.b >= b0 + 32) { b0 = at.b; hold(); }
+                if (at.b >= b0 + held) {
+                    b0 = at.b;
+                    held = 32;
+                    sq_l = b0 + lane < a.B ? tree_seq(a.cu_q, a.seq_start, b0 + lane, a.N, a.width) : TreeSeq{0, 0, 0, 0};
+                    w_l = tt_work(a, sq_l, G);
+                }
                 const int src = at.b - b0, np = __shfl_sync(0xffffffffu, w_l.np, src), tiles = __shfl_sync(0xffffffffu, w_l.tiles, src);
                 if (at.rb >= tiles * a.nkv) { ++at.b; at.rb = at.page = 0; continue; }
                 const bool ends = at.b == to.b && at.rb == to.rb;
@@ -314,10 +285,9 @@ attn_tree_tc_kernel(const TreeTc t) {
             if (x.npages == 0) break;
             const int* bt = a.block_table + (size_t)x.b * a.bt_stride + x.pg0;
             const uint32_t first = cv, end = cv + x.npages;
-            bool q_here = false;
             int ids = 0, before = 0;                    // page numbers 32 at a time, and the ones before them
             uint32_t spin = 0;
-            while (cv < end || !q_here) {
+            while (cv < end) {
                 // whichever slot is free: K tiles run ahead of V tiles, their slots come free earlier
                 if (ck < end && tt_warp_test(&k_empty[ck % TT_STAGES], ((ck / TT_STAGES) & 1) ^ 1)) {
                     const uint32_t i = ck - first, st = ck % TT_STAGES;
@@ -345,12 +315,6 @@ attn_tree_tc_kernel(const TreeTc t) {
                     ++cv;
                     spin = 0;
                 }
-                // half of Q, when the S product of the page before this unit has given its slot back (it was the last to read Q)
-                if (!q_here && ck > first && tt_warp_test(&k_empty[(first + 1) % TT_STAGES], (((first + 1) / TT_STAGES) & 1) ^ 1)) {
-                    gather_q(x, 0);
-                    q_here = true;
-                    spin = 0;
-                }
                 if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
             }
         }
@@ -375,10 +339,24 @@ attn_tree_tc_kernel(const TreeTc t) {
             const TreeUnit x = unit_at(slot);
             const uint32_t first = cv, end = cv + x.npages;
             if (x.npages == 0) break;
-            // half of Q, once the last unit's S products have read theirs; the other half is warp 0's
+            // Q into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7), once the last unit's S products have read theirs. Rows
+            // that the sequence has not keep what was there: they are nobody's.
             if (cs > 0 && !(ok = tt_warp_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1))) break;
-            gather_q(x, 1);
-            if (!(ok = tt_warp_wait(q_ready, k & 1))) break;
+            const int nrows = min(PT_ROWS, x.q * G - x.f0), pieces = kw >> 3, rows = 32 / pieces, piece = lane % pieces;
+            if (lane < rows * pieces) {
+                int row = lane / pieces, tok = (x.f0 + row) / G, h = x.f0 + row - tok * G;
+                for (; row < nrows; row += rows) {
+                    const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + ((size_t)(x.n0 + tok) * a.nq + x.kvh * G + h) * kw + 8 * piece;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_at + (piece >> 3) * (PT_ROWS * 128) + row * 128 +
+                                                                                   (((piece & 7) ^ (row & 7)) << 4)), "l"(src)
+                                 : "memory");
+                    h += rows;
+                    while (h >= G) { h -= G; ++tok; }
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the tensor cores read it
+            __syncwarp();
             uint32_t spin = 0;
             while (cv < end) {
                 // S of the next page as soon as its keys are there (its buffer's last weights went into a product that was
@@ -708,7 +686,7 @@ attn_tree_tc_join_kernel(const TreeTc t, int blocks) {
 // What a call's blocks need: shared memory, blocks that are resident at once (and no more than the work can come to, whatever the
 // lengths are), and float32 numbers of scratch: two partial results a block and the cuts.
 static int tt_smem(int d, int dv) {
-    const int smem = PT_ROWS * d * 2 + TT_STAGES * LUMEN_PAGE * (d + dv) * 2 + TT_BAR_WORDS * 8 + (TT_THREADS + 1) * 8;
+    const int smem = PT_ROWS * d * 2 + TT_STAGES * LUMEN_PAGE * (d + dv) * 2 + TT_BAR_WORDS * 8;
     return dv > 128 && smem < 116 * 1024 ? 116 * 1024 : smem;        // values beyond 128: all of the SM's tensor memory for one block
 }
 static int tt_blocks(int B, int N, int width, int nq, int nkv, int d, int dv) {
@@ -732,8 +710,10 @@ static cudaError_t tt_go(const TreeTc& t, int blocks, cudaStream_t stream) {
 }
 
 // Whether the kernel takes these arguments (beside the operands' places, which bulk copies and its wide stores need).
-static bool tt_takes(int is_bf16, int d, int dv, int layout, int v_layout, float scale) {
-    return is_bf16 && layout == LUMEN_LAYOUT_SW128 && v_layout == LUMEN_LAYOUT_SW128 && d <= 256 && dv <= 256 && scale > 0.0f;
+static bool tt_takes(int is_bf16, int B, int N, int width, int nq, int nkv, int d, int dv, int layout, int v_layout, float scale) {
+    // the work and a sequence's rows are counted in 32 bits
+    const long long work = ((long long)N * (nq / nkv) / PT_ROWS + B) * nkv * ((long long)width + TT_COST);
+    return work < (1 << 30) && (long long)N * (nq / nkv) < (1 << 30) && is_bf16 && layout == LUMEN_LAYOUT_SW128 && v_layout == LUMEN_LAYOUT_SW128 && d <= 256 && dv <= 256 && scale > 0.0f;
 }
 static bool tt_aligned(const void* q, const void* kcache, const void* vcache, const void* out) {
     return !(((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache) & 15) && !((uintptr_t)out & 31);

@@ -2073,7 +2073,8 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
     width = block_table.shape[1]
     bf16 = _is_bf16(q)
     where = (ptr(q), ptr(kcache), ptr(vcache), ptr(out))
-    tc = int_fn("attn_tree", "lumen_attn_tree_tc", [P] * 4 + [c_int] * 5 + [c_float])(*where, bf16, d, dv, layout, v_layout, scale)
+    tc = int_fn("attn_tree", "lumen_attn_tree_tc", [P] * 4 + [c_int] * 10 + [c_float])(
+        *where, bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale)
     scratch_k = int_fn("attn_tree", "lumen_attn_tree_scratch", [c_int] * 8)(tc, B, N, width, nq, nkv, d, dv)
     scratch = torch.empty((max(scratch_k, 0) * 1024,), dtype=F32, device=q.device) if scratch_k else None
     f = fn("attn_tree", "lumen_attn_tree",
