@@ -91,6 +91,7 @@ __device__ __forceinline__ bool tt_elect() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p)::"memory");
     return p != 0;
 }
+__device__ __forceinline__ void tt_prefetch(const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); }
 // 32 bytes in one instruction; to has to lie on 32 bytes.
 __device__ __forceinline__ void tt_store32(void* to, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
@@ -219,6 +220,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                     const TreeSeq s = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
                     s_first[0] = s.n0; s_first[1] = s.q; s_first[2] = s.start; s_first[3] = s.end;
                     s_first[4] = w.pg_lo; s_first[5] = w.np; s_first[6] = w.tiles;
+                    tt_prefetch(a.block_table + (size_t)cut.b * a.bt_stride + w.pg_lo + cut.page);
                 }
             }
         }
@@ -333,27 +335,37 @@ attn_tree_tc_kernel(const TreeTc t) {
         const uint32_t q_at = smem_u32(sQ), kv_at = smem_u32(sKV);
         bool ok = true;
         uint32_t cs = 0, cv = 0;                        // pages whose S, whose O product has been issued
+        // Q of a unit into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7): a node's G rows lie together in memory. Rows that
+        // the sequence has not keep what was there: they are nobody's.
+        auto ask_q = [&](const TreeUnit& x) {
+            const int nrows = min(PT_ROWS, x.q * G - x.f0), pieces = kw >> 3, tok0 = x.f0 / G, skip = x.f0 - tok0 * G;
+            const int toks = (skip + nrows + G - 1) / G;
+            const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + ((size_t)(x.n0 + tok0) * a.nq + x.kvh * G) * kw;
+            for (int i = lane; i < G * pieces; i += 32) {
+                const int h = i / pieces, c = i - h * pieces;
+                const uint32_t to = q_at + (c >> 3) * (PT_ROWS * 128);
+                const __nv_bfloat16* from = src + 8 * i;
+                int row = h - skip;
+#pragma unroll 4
+                for (int tok = 0; tok < toks; ++tok, row += G, from += (size_t)a.nq * kw)
+                    if (row >= 0 && row < nrows)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(from)
+                                     : "memory");
+            }
+        };
+        bool asked = false;                             // whether the next unit's Q is under way
         for (int k = 0; ok; ++k) {
             const int slot = k & 1;
             if (!(ok = tt_warp_wait(&u_full[slot], (k >> 1) & 1))) break;
             const TreeUnit x = unit_at(slot);
             const uint32_t first = cv, end = cv + x.npages;
             if (x.npages == 0) break;
-            // Q into [kw/64][row][64], 16-byte chunk c of a row at c ^ (row & 7), once the last unit's S products have read theirs. Rows
-            // that the sequence has not keep what was there: they are nobody's.
-            if (cs > 0 && !(ok = tt_warp_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1))) break;
-            const int nrows = min(PT_ROWS, x.q * G - x.f0), pieces = kw >> 3, rows = 32 / pieces, piece = lane % pieces;
-            if (lane < rows * pieces) {
-                int row = lane / pieces, tok = (x.f0 + row) / G, h = x.f0 + row - tok * G;
-                for (; row < nrows; row += rows) {
-                    const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + ((size_t)(x.n0 + tok) * a.nq + x.kvh * G + h) * kw + 8 * piece;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_at + (piece >> 3) * (PT_ROWS * 128) + row * 128 +
-                                                                                   (((piece & 7) ^ (row & 7)) << 4)), "l"(src)
-                                 : "memory");
-                    h += rows;
-                    while (h >= G) { h -= G; ++tok; }
-                }
+            if (!asked) {
+                // the last unit's S products have read their Q
+                if (cs > 0 && !(ok = tt_warp_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1))) break;
+                ask_q(x);
             }
+            asked = false;
             asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the tensor cores read it
             __syncwarp();
@@ -391,6 +403,13 @@ attn_tree_tc_kernel(const TreeTc t) {
                     }
                     __syncwarp();
                     ++cv;
+                    spin = 0;
+                } else if (!asked && cs == end && tt_warp_test(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1) &&
+                           tt_warp_test(&u_full[slot ^ 1], ((k + 1) >> 1) & 1)) {
+                    // all S products are done, the last weights are not yet: time for the next unit's Q
+                    const TreeUnit next = unit_at(slot ^ 1);
+                    if (next.npages > 0) ask_q(next);
+                    asked = true;
                     spin = 0;
                 } else if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) {
                     ok = false;
@@ -434,6 +453,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                 lo_last = max(0, __reduce_max_sync(0xffffffffu, top) - a.window + 1);
             }
             auto masked = [&](int jb) { return jb + LUMEN_PAGE > sq.start || jb < lo_last; };      // the same for every row
+            if ((pg0 + npages) * LUMEN_PAGE > sq.start) tt_prefetch(mask);
             bool any_masked = false;
             float m_ref = -INFINITY, l = 0.0f;
             for (int it = 0; it < npages; ++it, ++c) {
@@ -456,28 +476,27 @@ attn_tree_tc_kernel(const TreeTc t) {
                         s[j] = (s0 >> j) & 1 ? s[j] : -INFINITY;
                         s[32 + j] = (s1 >> j) & 1 ? s[32 + j] : -INFINITY;
                     }
-                    // this thread's half of a value row, in every block of 64 numbers
-                    const int st = c % TT_STAGES, vr = (threadIdx.x - 64) >> 1, half = threadIdx.x & 1;
+                    // values that are no numbers: 16 bytes a thread at a time, neighbours' side by side
+                    const int st = c % TT_STAGES;
                     if (!tt_warp_wait(&v_full[st], (c / TT_STAGES) & 1)) { ok = false; break; }
-                    unsigned char* row = sKV + st * STAGE_BYTES + K_BYTES + vr * 128 + half * 64;
+                    uint4* tile = reinterpret_cast<uint4*>(sKV + st * STAGE_BYTES + K_BYTES);
                     bool bad = false;
-                    for (int blk = 0; blk < vw >> 6; ++blk) {
-                        uint4* y = reinterpret_cast<uint4*>(row + blk * (LUMEN_PAGE * 128));
+#pragma unroll 4
+                    for (int i = threadIdx.x - 64; i < V_BYTES / 16; i += 128) {
+                        uint4 v = tile[i];
+                        uint32_t* p = reinterpret_cast<uint32_t*>(&v);
+                        bool here = false;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 v = y[i];
-                            uint32_t* p = reinterpret_cast<uint32_t*>(&v);
-                            bool here = false;
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {            // exponents of all ones
-                                if ((p[h] & 0x7f80u) == 0x7f80u) { p[h] &= 0xffff0000u; here = true; }
-                                if ((p[h] & 0x7f800000u) == 0x7f800000u) { p[h] &= 0x0000ffffu; here = true; }
-                            }
-                            if (here) y[i] = v;
-                            bad |= here;
+                        for (int h = 0; h < 4; ++h) {                // exponents of all ones
+                            if ((p[h] & 0x7f80u) == 0x7f80u) { p[h] &= 0xffff0000u; here = true; }
+                            if ((p[h] & 0x7f800000u) == 0x7f800000u) { p[h] &= 0x0000ffffu; here = true; }
+                        }
+                        if (here) {
+                            tile[i] = v;
+                            bad |= jb + ((i >> 3) & (LUMEN_PAGE - 1)) < sq.end;
                         }
                     }
-                    if (bad && jb + vr < sq.end) s_bad[k & 1] = k + 1;         // every writer writes the same
+                    if (bad) s_bad[k & 1] = k + 1;               // every writer writes the same
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
