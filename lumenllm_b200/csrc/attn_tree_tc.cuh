@@ -36,13 +36,18 @@
 // A place in the step's work: page `page` (counted from the first that the sequence's nodes see) of row block rb of sequence b.
 // b = B: the end.
 struct TreeCut {
-    int b, rb, page, unused;
+    int b, rb, page;
+};
+// A row block that is cut, as each of its cuts leaves it for the second kernel: its sequence's first token, its first row, kv head and
+// rows, the pieces it is in (0: this cut lies between row blocks) and the number of this cut among its own.
+struct TreeJoin {
+    int n0, f0, kvh, nrows, pieces, order, unused[2];
 };
 struct TreeTc {
     TreeArgs a;
     float scale_log2;             // with CAP softcap * log2(e), what the tanh is multiplied by
     float cap_pre;                // with CAP scale / softcap
-    TreeCut* cuts;                // [blocks] where their work begins
+    TreeJoin* joins;              // [blocks] the row blocks that their work begins inside of
     int* err;
 };
 // A unit: rows f0 .. f0 + 127 of sequence b and kv head kvh over pages pg0 .. pg0 + npages - 1 (npages 0: there is no more). slot: where
@@ -190,7 +195,7 @@ attn_tree_tc_kernel(const TreeTc t) {
 #pragma unroll 1
         for (int end = 0; end < 2; ++end) {
             int x = ((int)blockIdx.x + end) * share;
-            TreeCut cut = {a.B, 0, 0, 0};
+            TreeCut cut = {a.B, 0, 0};
             if (x >= total ? threadIdx.x != 0 : x < sum || x >= sum + mine) continue;
             if (x < total) {
                 x -= sum;
@@ -213,16 +218,24 @@ attn_tree_tc_kernel(const TreeTc t) {
                 }
             }
             s_cut[end] = cut;
-            if (end == 0) {
-                t.cuts[blockIdx.x] = cut;
-                // what warp 0 needs for the block's first keys
-                if (cut.b < a.B) {
-                    const TreeSeq s = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
-                    s_first[0] = s.n0; s_first[1] = s.q; s_first[2] = s.start; s_first[3] = s.end;
-                    s_first[4] = w.pg_lo; s_first[5] = w.np; s_first[6] = w.tiles;
-                    tt_prefetch(a.block_table + (size_t)cut.b * a.bt_stride + w.pg_lo + cut.page);
+            if (end == 1) continue;
+            TreeJoin join = {0, 0, 0, 0, 0, 0, {0, 0}};
+            if (cut.b < a.B) {
+                // what warp 0 needs for the block's first keys, and the second kernel to put the row block together
+                const TreeSeq s = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
+                s_first[0] = s.n0; s_first[1] = s.q; s_first[2] = s.start; s_first[3] = s.end;
+                s_first[4] = w.pg_lo; s_first[5] = w.np; s_first[6] = w.tiles;
+                tt_prefetch(a.block_table + (size_t)cut.b * a.bt_stride + w.pg_lo + cut.page);
+                if (cut.page > 0) {
+                    join.n0 = s.n0;
+                    join.kvh = cut.rb / w.tiles;
+                    join.f0 = (cut.rb - join.kvh * w.tiles) * PT_ROWS;
+                    join.nrows = min(PT_ROWS, s.q * G - join.f0);
+                    join.order = (cut.page - 2) / share;          // the cuts before it and behind it lie `share` pages apart
+                    join.pieces = 2 + join.order + (w.np - 2 - cut.page) / share;
                 }
             }
+            t.joins[blockIdx.x] = join;
         }
     }
     __syncthreads();
@@ -641,69 +654,64 @@ attn_tree_tc_kernel(const TreeTc t) {
     }
 }
 
-// Joins the pieces of the row blocks that were cut. Blocks x = i - 1 have the cut where block i of the kernel before began its work: the
-// first cut of a row block joins all of its pieces, in the order of their pages; a thread has four columns of a row.
-__global__ void __launch_bounds__(256)
-attn_tree_tc_join_kernel(const TreeTc t, int blocks) {
+// Joins the pieces of the row blocks that were cut, in the order of their pages; the blocks of all of its
+// cuts share a row block's rows, a thread has four columns of a row at a time. What it takes is the latency of its loads, one behind
+// the other: those of TJ_BATCH pieces are under way together, and few registers let all blocks be resident at once.
+#define TJ_BATCH 4
+#define TJ_SLICES 4               // blocks a cut
+__global__ void __launch_bounds__(256, 4)
+attn_tree_tc_join_kernel(const TreeTc t) {
     pdl_wait();
     pdl_trigger();
     const TreeArgs& a = t.a;
-    const int i = blockIdx.x + 1, lane = threadIdx.x & 31;
-    const TreeCut cut = t.cuts[i], before = t.cuts[i - 1];
-    if (cut.page == 0 || (before.page > 0 && before.b == cut.b && before.rb == cut.rb)) return;
-    const int G = a.nq / a.nkv;
-    const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
-    const int tiles = tt_work(a, sq, G).tiles, kvh = cut.rb / tiles, f0 = (cut.rb - kvh * tiles) * PT_ROWS;
-    const int quads = a.dv >> 2, idx = blockIdx.y * 256 + threadIdx.x, row = idx / quads, e = (idx - row * quads) * 4;
-    int pieces = 2;                                     // block i - 1's and block i's, and of those that begin in this row block too
-    for (int j = i + 1; j < blocks; j += 32) {
-        TreeCut c = {-1, 0, 0, 0};
-        if (j + lane < blocks) c = t.cuts[j + lane];
-        const unsigned out = __ballot_sync(0xffffffffu, !(c.b == cut.b && c.rb == cut.rb && c.page > 0));
-        pieces += out ? __ffs(out) - 1 : 32;
-        if (out) break;
-    }
-    if (row >= min(PT_ROWS, sq.q * G - f0)) return;
-    constexpr int BATCH = 8;                            // pieces whose loads are under way together
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f, top = -INFINITY;
-    for (int s0 = 0; s0 < pieces; s0 += BATCH) {
-        float2 x[BATCH];
-        float4 v[BATCH];
+    const int i = blockIdx.x + 1, G = a.nq / a.nkv, quads = a.dv >> 2;
+    const TreeJoin join = t.joins[i];
+    if (join.pieces == 0) return;
+    const size_t first = (size_t)(2 * (i - join.order) - 1) * PT_ROWS;       // piece 0: slot 1 of the block before the first cut
+    for (int idx = (join.order * TJ_SLICES + blockIdx.y) * 256 + threadIdx.x; idx < join.nrows * quads; idx += (join.pieces - 1) * TJ_SLICES * 256) {
+        const int row = idx / quads, e = (idx - row * quads) * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f, top = -INFINITY;
+        for (int s0 = 0; s0 < join.pieces; s0 += TJ_BATCH) {
+            float2 x[TJ_BATCH];
+            float4 v[TJ_BATCH];
 #pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-            x[s] = make_float2(-INFINITY, 0.0f);
-            v[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (s0 + s < pieces) {
-                const size_t at = (size_t)(2 * (i - 1 + s0 + s) + (s0 + s == 0 ? 1 : 0)) * PT_ROWS + row;
-                x[s] = a.part_ml[at];
-                v[s] = *reinterpret_cast<const float4*>(a.part_o + at * a.dv + e);
+            for (int s = 0; s < TJ_BATCH; ++s) {
+                x[s] = make_float2(-INFINITY, 0.0f);
+                v[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (s0 + s < join.pieces) {
+                    // the pieces behind: slot 0 of the block behind the first cut and of those that follow
+                    const size_t from = first + row + (s0 + s == 0 ? 0 : (size_t)(2 * (s0 + s) - 1) * PT_ROWS);
+                    x[s] = a.part_ml[from];
+                    v[s] = *reinterpret_cast<const float4*>(a.part_o + from * a.dv + e);
+                }
+            }
+            float mn = top;
+#pragma unroll
+            for (int s = 0; s < TJ_BATCH; ++s) mn = fmaxf(mn, x[s].x);
+            // weights in units of log 2; without a maximum there is no weight, or a score that is no number
+            const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(top - mn);
+            o.x *= c; o.y *= c; o.z *= c; o.w *= c;
+            l *= c;
+            top = mn;
+#pragma unroll
+            for (int s = 0; s < TJ_BATCH; ++s) {
+                if (x[s].x == -INFINITY && x[s].y == 0.0f) continue;
+                const float f = x[s].x == -INFINITY ? 1.0f : exp2f(x[s].x - mn);
+                o.x = fmaf(f, v[s].x, o.x); o.y = fmaf(f, v[s].y, o.y);
+                o.z = fmaf(f, v[s].z, o.z); o.w = fmaf(f, v[s].w, o.w);
+                l = fmaf(f, x[s].y, l);
             }
         }
-        float mn = top;
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s) mn = fmaxf(mn, x[s].x);
-        // weights in units of log 2; without a maximum there is no weight, or a score that is no number
-        const float c = top == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(top - mn);
-        o.x *= c; o.y *= c; o.z *= c; o.w *= c;
-        l *= c;
-        top = mn;
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-            if (x[s].x == -INFINITY && x[s].y == 0.0f) continue;
-            const float f = x[s].x == -INFINITY ? 1.0f : exp2f(x[s].x - mn);
-            o.x = fmaf(f, v[s].x, o.x); o.y = fmaf(f, v[s].y, o.y); o.z = fmaf(f, v[s].z, o.z); o.w = fmaf(f, v[s].w, o.w);
-            l = fmaf(f, x[s].y, l);
-        }
+        const int f = join.f0 + row, node = f / G, head = join.kvh * G + f - node * G;
+        const float inv = ta_close(top * 0.6931471805599453f, l, a.sink, head);
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(join.n0 + node) * a.nq + head) * a.dv + e) =
+            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
-    const int f = f0 + row, head = kvh * G + f % G;
-    const float inv = ta_close(top * 0.6931471805599453f, l, a.sink, head);
-    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv + e) =
-        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
 // What a call's blocks need: shared memory, blocks that are resident at once (and no more than the work can come to, whatever the
-// lengths are), and float32 numbers of scratch: two partial results a block and the cuts.
+// lengths are), and float32 numbers of scratch: two partial results a block and what to join.
 static int tt_smem(int d, int dv) {
     const int smem = PT_ROWS * d * 2 + TT_STAGES * LUMEN_PAGE * (d + dv) * 2 + TT_BAR_WORDS * 8;
     return dv > 128 && smem < 116 * 1024 ? 116 * 1024 : smem;        // values beyond 128: all of the SM's tensor memory for one block
@@ -714,7 +722,7 @@ static int tt_blocks(int B, int N, int width, int nq, int nkv, int d, int dv) {
     const long long n = (work + TT_SHARE - 1) / TT_SHARE;
     return (int)(n < most ? n : most);
 }
-static long long tt_floats(int blocks, int dv) { return (long long)blocks * (2 * PT_ROWS * (dv + 2) + 4); }
+static long long tt_floats(int blocks, int dv) { return (long long)blocks * (2 * PT_ROWS * (dv + 2) + 8); }
 
 template <int D, bool CAP>
 static cudaError_t tt_go(const TreeTc& t, int blocks, cudaStream_t stream) {
@@ -724,7 +732,7 @@ static cudaError_t tt_go(const TreeTc& t, int blocks, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) e = lumen_launch(k, dim3(blocks), dim3(TT_THREADS), smem, stream, t);
     if (e == cudaSuccess && blocks > 1)
-        e = lumen_launch(attn_tree_tc_join_kernel, dim3(blocks - 1, PT_ROWS * a.dv / 1024), dim3(256), 0, stream, t, blocks);
+        e = lumen_launch(attn_tree_tc_join_kernel, dim3(blocks - 1, TJ_SLICES), dim3(256), 0, stream, t);
     return e;
 }
 
@@ -744,7 +752,7 @@ static cudaError_t tt_launch(TreeArgs a, float* scratch, int* err, cudaStream_t 
     a.part_ml = (float2*)(scratch + rows * a.dv);
     const bool cap = a.softcap > 0.0f;
     const TreeTc t = {a, (cap ? a.softcap : a.scale) * 1.4426950408889634f, cap ? a.scale / a.softcap : 0.0f,
-                      (TreeCut*)(scratch + rows * (a.dv + 2)), err};
+                      (TreeJoin*)(scratch + rows * (a.dv + 2)), err};
 #define TT_GO(D) (cap ? tt_go<D, true>(t, blocks, stream) : tt_go<D, false>(t, blocks, stream))
     if (a.d == 128 && a.dv == 128) return TT_GO(128);
     if (a.d == 64 && a.dv == 64) return TT_GO(64);
