@@ -99,6 +99,9 @@ class CacheGroup:
         else:  # bookkeeping only (host tests)
             self.k = self.v = None
         self.table = np.zeros((max_slots, max_pages_per_seq), dtype=np.int32)
+        self.device = device
+        self._table_dev = None          # the table on the device, for steps that build their own there
+        self._changed = set()           # slots whose rows there are out of date
         # pages held by a slot: [0, kept) and [first_page, end_page), where kept covers the
         # first tokens a window keeps in sight (none without such tokens) and never gives back
         self.keep_pages = pages_for(need.keep_first) if (need.window > 0 or need.chunk > 0) else 0
@@ -122,6 +125,7 @@ class CacheGroup:
             except CacheFull as e:
                 raise CacheFull(f"slot {slot}: the cache is full ({e})") from None
             self.table[slot, have_end:want_end] = got
+            self._changed.add(slot)
             self.n_held[slot] += want_end - have_end
             self.end_page[slot] = want_end
 
@@ -140,6 +144,7 @@ class CacheGroup:
             n = first_needed - first
             self.pool.give_back(self.table[slot, first:first + n].tolist())
             self.table[slot, first:first + n] = 0
+            self._changed.add(slot)
             self.first_page[slot] = first + n
             self.n_held[slot] -= n
 
@@ -148,9 +153,24 @@ class CacheGroup:
         if held.size:
             self.pool.give_back(held.tolist())
         self.table[slot, :] = 0
+        self._changed.add(slot)
         self.first_page[slot] = 0
         self.end_page[slot] = 0
         self.n_held[slot] = 0
+
+
+    def device_table(self) -> torch.Tensor:
+        """The slots' pages on the device, int32 [max_slots, pages]: rows that have changed since the last call are
+        copied there, in the order of the current stream."""
+        if self._table_dev is None:
+            self._table_dev = torch.from_numpy(self.table.copy()).to(self.device)
+        elif self._changed:
+            rows = sorted(self._changed)
+            at = torch.tensor(rows, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
+            new = torch.from_numpy(self.table[rows]).pin_memory().to(self.device, non_blocking=True)
+            self._table_dev.index_copy_(0, at, new)
+        self._changed.clear()
+        return self._table_dev
 
 
 class StateStore:

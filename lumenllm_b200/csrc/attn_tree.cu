@@ -363,10 +363,10 @@ static int ta_segs(int width) {
     return n < TREE_MAX_SEGS ? n : TREE_MAX_SEGS;
 }
 
-// Which kernel a call takes: 1 the tensor cores'.
-LUMEN_API int lumen_attn_tree_tc(const void* q, const void* kcache, const void* vcache, const void* out, int is_bf16, int B, int N,
-                                 int width, int nq, int nkv, int d, int dv, int layout, int v_layout, float scale) {
-    return nkv > 0 && nq >= nkv && tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale) && tt_aligned(q, kcache, vcache, out) ? 1 : 0;
+// Which kernel a call takes whose operands lie on 16 bytes and its output on 32: 1 the tensor cores' (positive: the scale is above 0).
+LUMEN_API int lumen_attn_tree_tc(int is_bf16, int B, int N, int width, int nq, int nkv, int d, int dv, int layout, int v_layout,
+                                 int positive) {
+    return nkv > 0 && nq >= nkv && tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, positive ? 1.0f : 0.0f) ? 1 : 0;
 }
 // Thousands (1,024s) of float32 numbers of scratch that a call needs, -1: more than there can be.
 LUMEN_API int lumen_attn_tree_scratch(int tc, int B, int N, int width, int nq, int nkv, int d, int dv) {

@@ -35,6 +35,16 @@ class StepEntry:
     positions: Optional[Sequence[int]] = None
 
 
+@dataclass
+class DraftEntry:
+    """One sequence of a step that checks drafts: its slot, the tokens of a tree and the parent of each, a number of an
+    earlier one. tokens[0] is certain (the token that was sampled last and is not in the cache yet; parents[0] is
+    -1); the others are drafted: a path from the first down is a continuation that may be accepted."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
 def _pad4(n: int) -> int:
     return (n + 3) & ~3
 
@@ -60,6 +70,7 @@ class StepContext:
     cache: object = None
     n_real: Optional[int] = None   # sequences that are not padding
     extras: Dict[str, object] = field(default_factory=dict)
+    tree_mask: Optional[torch.Tensor] = None   # a step of drafts: which tokens of its sequence each token sees
 
     @property
     def is_decode(self) -> bool:
@@ -243,3 +254,34 @@ def build_context(cache, runtime, entries, meta_dev=None, pad_to: int = 0, table
         meta_dev = torch.empty((grow,), dtype=torch.int32, device=runtime.device)
     upload(host, meta_dev)
     return context_on(meta_dev[:lay.total], lay, q_lens, starts, slots, n_real, cache, runtime), meta_dev
+
+
+def tree_context(cache, runtime, entries: Sequence[DraftEntry]):
+    """The context of a step that checks drafts. The host sends the tokens, their parents, the slots and the lengths; the
+    rest is built on the device (ops.kernels.step_tables). Wanted are the logits at every token. Returns (context,
+    parents on the device); the cache has room for the tokens, nothing is committed."""
+    from ..ops import kernels as K
+    starts = [cache.reserve(e.slot, len(e.tokens)) for e in entries]
+    q_lens = [len(e.tokens) for e in entries]
+    B, N, longest = len(entries), sum(q_lens), max(q_lens)
+    width = max(pages_for(s + q) for s, q in zip(starts, q_lens))
+    offs = np.cumsum([0] + [_pad4(n) for n in (N, N, N, B, B, B)]).tolist()
+    host = np.zeros((offs[-1],), dtype=np.int32)
+    host[offs[0]:offs[0] + N] = np.concatenate([np.asarray(e.tokens, dtype=np.int64) for e in entries])
+    host[offs[1]:offs[1] + N] = np.concatenate([np.asarray(e.parents, dtype=np.int64) for e in entries])
+    host[offs[2]:offs[2] + N] = np.arange(N)
+    host[offs[3]:offs[3] + B] = [e.slot for e in entries]
+    host[offs[4]:offs[4] + B] = starts
+    host[offs[5]:offs[5] + B] = q_lens
+    dev = torch.empty((host.size,), dtype=torch.int32, device=runtime.device)
+    upload(host, dev)
+    tokens, parents, want = (dev[o:o + N] for o in offs[:3])
+    seq_slot, seq_start, seq_qlen = (dev[o:o + B] for o in offs[3:6])
+    tables = [K.step_tables(seq_start, seq_qlen, g.device_table(), seq_slot, N, width, parents=parents, mask_words=-(-longest // 64))
+              for g in cache.groups]
+    t = tables[0]
+    ctx = StepContext(
+        runtime=runtime, B=B, N=N, q_lens=q_lens, starts=starts, slots=[e.slot for e in entries], tokens=tokens,
+        rope_pos=t.tok_pos, cache_pos=t.cache_pos, tok_seq=t.tok_seq, seq_slot=seq_slot, seq_start=seq_start, seq_qlen=seq_qlen,
+        cu_q=t.cu_q, want_rows=want, block_tables=[x.block_table for x in tables], cache=cache, n_real=B, tree_mask=t.tree_mask)
+    return ctx, parents

@@ -26,7 +26,7 @@ from ..config import ConfigError, ModelSpec, load_config
 from ..ops import kernels as K
 from ..ops.native import KernelError
 from ..parts.base import Runtime
-from .context import StepContext, StepEntry, build_context
+from .context import DraftEntry, StepContext, StepEntry, build_context, tree_context
 from .model import DecoderModel, expected_tensors, tensor_fallbacks
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32,
@@ -244,6 +244,70 @@ class Engine:
         if cur:
             parts.append(cur)
         return parts, origin
+
+    # ------------------------------------------------------------ drafts
+    def verify(self, drafts: Sequence[DraftEntry], configs=None, uniforms=None) -> List[List[int]]:
+        """Checks drafted tokens of several sequences in one step. The model runs over every token of every tree, a token is
+        picked at each as generation picks it, and of the drafts those are kept that lie on the path of picked tokens
+        from the tree's first token down. Returns the next tokens of each sequence, in the order of the drafts: those kept and
+        the one picked behind the last of them, so one at least. The cache then holds the first token and the kept
+        ones; the last returned token is not in it: it is the next step's first.
+        `configs`: a SamplingConfig a sequence (without: greedy). `uniforms`: for each sequence as many numbers in [0, 1)
+        as its tree is deep, number k for the token picked at depth k: with the numbers that single steps would have drawn,
+        the tokens are those of single steps (up to the rounding of logits)."""
+        drafts = [e if isinstance(e, DraftEntry) else DraftEntry(*e) for e in drafts]
+        depths = self._validate_drafts(drafts, configs, uniforms)
+        try:
+            ctx, parents = tree_context(self.cache, self.runtime, drafts)
+        except CacheFull as e:
+            raise StepError(str(e)) from e
+        logits = self.model.forward(ctx)
+        self.steps_run += 1
+        if configs is None:
+            picked = K.argmax(logits)
+        else:
+            picked = self.sampler.pick(logits, [c for c, d in zip(configs, depths) for _ in d],
+                                       [0.0 if u is None else float(u[x]) for u, d in
+                                        zip(uniforms or [None] * len(drafts), depths) for x in d])
+        count, path, emitted = K.tree_accept(picked, ctx.tokens, parents, ctx.cu_q, 1 + max(max(d) for d in depths))
+        for g, table in zip(self.cache.groups, ctx.block_tables):
+            K.cache_compact(g.k, None if g.need.values_in_keys else g.v, table, ctx.seq_start, path, count, layout=g.layout,
+                            v_layout=g.v_layout)
+        counts, out = count.tolist(), emitted.tolist()
+        self.check_kernels()
+        for e, n in zip(drafts, counts):
+            self.cache.commit(e.slot, n)
+        return [row[:n] for row, n in zip(out, counts)]
+
+    def _validate_drafts(self, drafts, configs, uniforms) -> List[List[int]]:
+        """Refuses what cannot be checked; returns every token's depth in its tree."""
+        if not self.model.tree_safe:
+            raise StepError("this model takes no drafts: one of its layers keeps state from token to token, or has an attention "
+                            "that no tree of tokens goes through")
+        self._validate([StepEntry(e.slot, e.tokens) for e in drafts])
+        if sum(len(e.tokens) for e in drafts) > self.max_step_tokens:
+            raise StepError(f"{sum(len(e.tokens) for e in drafts)} tokens of drafts exceed a step's {self.max_step_tokens}")
+        if configs is not None:
+            if len(configs) != len(drafts) or (uniforms is not None and len(uniforms) != len(drafts)):
+                raise StepError("one sampling config and one row of uniform numbers a sequence")
+            for c in configs:
+                c.validate()
+            if uniforms is None and not all(c.greedy for c in configs):
+                raise StepError("sampling needs uniform numbers")
+        depths = []
+        for i, e in enumerate(drafts):
+            n = len(e.tokens)
+            if n > K.TREE_MAX_NODES:
+                raise StepError(f"slot {e.slot}: {n} tokens, a tree has up to {K.TREE_MAX_NODES}")
+            if len(e.parents) != n or int(e.parents[0]) != -1 or any(not 0 <= int(p) < j for j, p in enumerate(e.parents) if j):
+                raise StepError(f"slot {e.slot}: parents are -1 for the first token and an earlier token's number for every other")
+            d = [0]
+            for p in e.parents[1:]:
+                d.append(d[int(p)] + 1)
+            if configs is not None and uniforms is not None and not configs[i].greedy and len(uniforms[i]) <= max(d):
+                raise StepError(f"slot {e.slot}: {len(uniforms[i])} uniform numbers for a tree {max(d) + 1} tokens deep")
+            depths.append(d)
+        return depths
 
     # ------------------------------------------------------------ generation
     def check_kernels(self) -> None:

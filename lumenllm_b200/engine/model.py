@@ -50,6 +50,9 @@ class DecoderModel:
         self.graph_safe = all(b.graph_safe if hasattr(b, "graph_safe") else
                               (getattr(b.mixer, "graph_safe", False) and getattr(b.ffn, "graph_safe", False))
                               for b in self.blocks)
+        # a step may bring trees of drafted tokens if every mixer takes them and no layer keeps state from token to token
+        self.tree_safe = (all(getattr(b.mixer, "tree_safe", False) for b in self.blocks) and not self.state_shapes()
+                          and bool(self.cache_needs()))
         # whether a token's sums depend on where its sequence's tokens of the step begin
         self.cut_matters = any(getattr(b.mixer, "cut_matters", False) for b in self.blocks)
 

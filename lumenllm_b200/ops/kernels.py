@@ -9,6 +9,7 @@ from __future__ import annotations
 
 from collections import namedtuple
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from functools import lru_cache
 
 import torch
 
@@ -1960,25 +1961,27 @@ TREE_MAX_NODES = 256      # nodes of a sequence that masks and walks cover: TREE
 StepTables = namedtuple("StepTables", "cu_q tok_seq cache_pos tok_pos slot_map block_table tree_mask")
 
 
-def _arrays(what, **tensors):
-    """Contiguous arrays of one type each, all on the current device: name=(tensor, dtype, numbers at least)."""
-    for name, (t, dtype, n) in tensors.items():
-        if t.dtype != dtype:
+def _arrays(what, *arrays):
+    """Contiguous arrays of one type each, all on the current device: (name, tensor, dtype, numbers at least). A step makes these
+    calls once a layer, and a short step waits for them: the good case is a few comparisons a tensor."""
+    for name, t, dtype, n in arrays:
+        if t.dtype is not dtype:
             raise KernelError(f"{what}.{name}: expected {dtype}, got {t.dtype}")
         if t.numel() < n:
             raise KernelError(f"{what}.{name}: {t.numel()} numbers, {n} are needed")
         if not t.is_contiguous():
             raise KernelError(f"{what}.{name}: tensor must be contiguous")
-    _here(what, [t for t, _, _ in tensors.values()])
+    _here(what, *[x[1] for x in arrays])
 
 
-def _here(what, tensors):
+def _here(what, *tensors):
     """All on a CUDA device, and on the current one (whose stream a launch goes to)."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise KernelError(f"{what}: a tensor is not on a CUDA device (no CPU path exists)")
-        if t.get_device() != torch.cuda.current_device():
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    at = {t.get_device() for t in tensors}
+    if -1 in at:
+        raise KernelError(f"{what}: a tensor is not on a CUDA device (no CPU path exists)")
+    current = torch.cuda.current_device()
+    if at != {current}:
+        raise KernelError(f"{what}: tensors on devices {sorted(at)}, the current device is {current}")
 
 
 def _page_table(what, block_table, rows):
@@ -1986,6 +1989,9 @@ def _page_table(what, block_table, rows):
             or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise KernelError(f"{what}.block_table: int32 [{rows} or more, pages] with dense rows is needed, not "
                           f"{tuple(block_table.shape)} of {block_table.dtype}")
+
+
+_STEP_TABLES_ARGS = [P, P, P, c_longlong, c_int, P, P, c_int, c_int, c_int, c_int, P, P, P, P, P, P, P, P]
 
 
 def step_tables(seq_start, seq_qlen, slot_pages, seq_slot, n_tokens, width, parents=None, mask_words=1):
@@ -2008,20 +2014,28 @@ def step_tables(seq_start, seq_qlen, slot_pages, seq_slot, n_tokens, width, pare
                           f"{tuple(slot_pages.shape)} of {slot_pages.dtype}")
     if N < 0 or not 1 <= width <= 1 << 24 or not 1 <= words <= TREE_MAX_NODES // 64:
         raise KernelError(f"step_tables: {N} tokens, {width} pages, {words} mask words")
-    _arrays("step_tables", seq_start=(seq_start, I32, B), seq_qlen=(seq_qlen, I32, B), seq_slot=(seq_slot, I32, B),
-            parents=(seq_start if parents is None else parents, I32, 0 if parents is None else N))
-    _here("step_tables", [slot_pages])
-    dev = seq_start.device
-    cu_q, tok_seq, cache_pos, tok_pos, table = torch.empty((B + 1 + 3 * N + (B + 1) * width,), dtype=I32, device=dev).split(
-        (B + 1, N, N, N, (B + 1) * width))
-    table = table.view(B + 1, width)
-    slot_map = torch.empty((N,), dtype=I64, device=dev)
-    mask = torch.empty((N, words), dtype=I64, device=dev) if parents is not None else None
-    f = fn("draft", "lumen_step_tables", [P, P, P, c_longlong, c_int, P, P, c_int, c_int, c_int, c_int, P, P, P, P, P, P, P, P])
+    _arrays("step_tables", ("seq_start", seq_start, I32, B), ("seq_qlen", seq_qlen, I32, B), ("seq_slot", seq_slot, I32, B),
+            ("parents", seq_start if parents is None else parents, I32, 0 if parents is None else N))
+    _here("step_tables", slot_pages)
+    new = seq_start.new_empty
+    cu_q, tok_seq, cache_pos, tok_pos = new((B + 1 + 3 * N,)).split((B + 1, N, N, N))
+    table, slot_map = new((B + 1, width)), new((N,), dtype=I64)
+    mask = new((N, words), dtype=I64) if parents is not None else None
+    f = fn("draft", "lumen_step_tables", _STEP_TABLES_ARGS)
     check(f(ptr(seq_start), ptr(seq_qlen), ptr(slot_pages), slot_pages.stride(0), slot_pages.shape[0], ptr(seq_slot), ptr(parents),
             B, N, width, words, ptr(cu_q), ptr(tok_seq), ptr(cache_pos), ptr(tok_pos), ptr(slot_map), ptr(table), ptr(mask),
             stream_ptr()), "step_tables")
     return StepTables(cu_q, tok_seq, cache_pos, tok_pos, slot_map, table, mask)
+
+
+_ATTN_TREE_ARGS = [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, c_int, P] + [c_int] * 10 + [c_float, c_float, P, c_int, c_int, P, P]
+
+
+@lru_cache(maxsize=4096)
+def _attn_tree_plan(aligned, bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, positive):
+    """(whether the tensor cores' kernel takes such a call, 1,024s of float32 numbers of scratch it needs)."""
+    tc = int_fn("attn_tree", "lumen_attn_tree_tc", [c_int] * 11)(bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, 1 if positive else 0) if aligned else 0
+    return tc, int_fn("attn_tree", "lumen_attn_tree_scratch", [c_int] * 8)(tc, B, N, width, nq, nkv, d, dv)
 
 
 def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos, tree_mask, window, scale,
@@ -2038,13 +2052,15 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
     not matter, infinities and NaN included. Rows behind the last sequence (cu_q[B]) are not written; `out` takes the result.
     Keys and values up to 512 numbers, any nq that is a multiple of nkv."""
     N, nq, d = q.shape
-    if q.dtype not in (F32, BF16) or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+    dtype = q.dtype
+    if (dtype is not BF16 and dtype is not F32) or kcache.dtype is not dtype or vcache.dtype is not dtype:
         raise KernelError(f"attn_tree: queries and caches are all float32 or all bfloat16, not {q.dtype}, {kcache.dtype}, {vcache.dtype}")
     if kcache.dim() != 4 or vcache.dim() != 4:
         raise KernelError("attn_tree: caches are [pages, kv heads, PAGE, size]")
-    n_pages, nkv, dv = kcache.shape[0], kcache.shape[1], vcache.shape[3]
+    n_pages, nkv, page, kd = kcache.shape
+    v_pages, v_nkv, v_page, dv = vcache.shape
     v_layout = layout if v_layout is None else v_layout
-    if tuple(kcache.shape[1:]) != (nkv, PAGE, d) or tuple(vcache.shape[:3]) != (n_pages, nkv, PAGE) or not nkv or nq % nkv or not nq:
+    if page != PAGE or v_page != PAGE or kd != d or v_pages != n_pages or v_nkv != nkv or not nkv or nq % nkv or not nq:
         raise KernelError(f"attn_tree: caches {tuple(kcache.shape)}, {tuple(vcache.shape)} do not fit {nq} queries of {d}")
     if not 1 <= d <= 512 or not 1 <= dv <= 512 or n_pages < 1:
         raise KernelError(f"attn_tree takes keys and values of 1 to 512 numbers, not {d} and {dv}")
@@ -2058,31 +2074,34 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
         raise KernelError(f"attn_tree: window {window}, softcap {softcap}, {B} sequences")
     _page_table("attn_tree", block_table, B)
     words = tree_mask.shape[1]
-    _arrays("attn_tree", q=(q, q.dtype, 0), kcache=(kcache, q.dtype, 0), vcache=(vcache, q.dtype, 0), cu_q=(cu_q, I32, 1),
-            seq_start=(seq_start, I32, B), tok_seq=(tok_seq, I32, N), tok_pos=(tok_pos, I32, N), tree_mask=(tree_mask, I64, N * words))
-    _here("attn_tree", [block_table])
+    _arrays("attn_tree", ("q", q, dtype, 0), ("kcache", kcache, dtype, 0), ("vcache", vcache, dtype, 0), ("cu_q", cu_q, I32, 1),
+            ("seq_start", seq_start, I32, B), ("tok_seq", tok_seq, I32, N), ("tok_pos", tok_pos, I32, N),
+            ("tree_mask", tree_mask, I64, N * words))
+    _here("attn_tree", block_table)
     if out is None:
-        out = torch.empty((N, nq, dv), dtype=q.dtype, device=q.device)
+        out = q.new_empty((N, nq, dv))
     elif tuple(out.shape) != (N, nq, dv):
         raise KernelError(f"attn_tree: out {tuple(out.shape)} is not {(N, nq, dv)}")
     else:
-        _arrays("attn_tree", out=(out, q.dtype, 0))
+        _arrays("attn_tree", ("out", out, dtype, 0))
     if N == 0 or B == 0:
         return out
     sink = _sink_arg(sink, nq, q.device)
     width = block_table.shape[1]
-    bf16 = _is_bf16(q)
-    where = (ptr(q), ptr(kcache), ptr(vcache), ptr(out))
-    tc = int_fn("attn_tree", "lumen_attn_tree_tc", [P] * 4 + [c_int] * 10 + [c_float])(
-        *where, bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale)
-    scratch_k = int_fn("attn_tree", "lumen_attn_tree_scratch", [c_int] * 8)(tc, B, N, width, nq, nkv, d, dv)
-    scratch = torch.empty((max(scratch_k, 0) * 1024,), dtype=F32, device=q.device) if scratch_k else None
-    f = fn("attn_tree", "lumen_attn_tree",
-           [P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, P, c_int, P] + [c_int] * 10 + [c_float, c_float, P, c_int, c_int, P, P])
-    check(f(*where[:3], ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq), ptr(tok_pos),
-            ptr(tree_mask), words, where[3], tc, ptr(scratch), scratch_k, bf16, B, N, n_pages, nq, nkv, d, dv, int(window), float(scale),
+    pq, pk, pv, po = q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr()
+    bf16 = 1 if dtype is BF16 else 0
+    # the tensor cores' kernel copies in pieces of 16 bytes and writes 32 at a time
+    aligned = not ((pq | pk | pv) & 15 or po & 31)
+    tc, scratch_k = _attn_tree_plan(aligned, bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale > 0.0)
+    scratch = q.new_empty((scratch_k * 1024,), dtype=F32) if scratch_k > 0 else None
+    f = fn("attn_tree", "lumen_attn_tree", _ATTN_TREE_ARGS)
+    check(f(pq, pk, pv, ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq), ptr(tok_pos),
+            ptr(tree_mask), words, po, tc, ptr(scratch), scratch_k, bf16, B, N, n_pages, nq, nkv, d, dv, int(window), float(scale),
             float(softcap), ptr(sink), int(layout), int(v_layout), ptr(error_flag(q.device)), stream_ptr()), "attn_tree")
     return out
+
+
+_TREE_ACCEPT_ARGS = [P, P, P, P, c_int, c_int, c_int, P, P, P, P]
 
 
 def tree_accept(picked, tokens, parents, cu_q, max_path):
@@ -2096,12 +2115,15 @@ def tree_accept(picked, tokens, parents, cu_q, max_path):
     N, B, most = picked.numel(), cu_q.numel() - 1, int(max_path)
     if B < 0 or not 1 <= most <= TREE_MAX_NODES:
         raise KernelError(f"tree_accept: {B} sequences, paths of up to {max_path} (1 to {TREE_MAX_NODES})")
-    _arrays("tree_accept", picked=(picked, I32, N), tokens=(tokens, I32, N), parents=(parents, I32, N), cu_q=(cu_q, I32, 1))
-    count, path, emitted = torch.empty((B * (1 + 2 * most),), dtype=I32, device=picked.device).split((B, B * most, B * most))
-    f = fn("draft", "lumen_tree_accept", [P, P, P, P, c_int, c_int, c_int, P, P, P, P])
+    _arrays("tree_accept", ("picked", picked, I32, N), ("tokens", tokens, I32, N), ("parents", parents, I32, N), ("cu_q", cu_q, I32, 1))
+    count, path, emitted = cu_q.new_empty((B,)), cu_q.new_empty((B, most)), cu_q.new_empty((B, most))
+    f = fn("draft", "lumen_tree_accept", _TREE_ACCEPT_ARGS)
     check(f(ptr(picked), ptr(tokens), ptr(parents), ptr(cu_q), B, N, most, ptr(count), ptr(path), ptr(emitted), stream_ptr()),
           "tree_accept")
-    return count, path.view(B, most), emitted.view(B, most)
+    return count, path, emitted
+
+
+_CACHE_COMPACT_ARGS = [P, P, P, c_int, c_int, P, P, c_int, P] + [c_int] * 9 + [P]
 
 
 def cache_compact(kcache, vcache, block_table, seq_start, path, count, layout=LAYOUT_LINEAR, v_layout=None):
@@ -2128,11 +2150,11 @@ def cache_compact(kcache, vcache, block_table, seq_start, path, count, layout=LA
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= TREE_MAX_NODES or B > 65535 or n_pages > 1 << 24:
         raise KernelError(f"cache_compact: path {tuple(path.shape)} for {B} sequences (1 to {TREE_MAX_NODES} tokens each)")
     _page_table("cache_compact", block_table, B)
-    _arrays("cache_compact", kcache=(kcache, kcache.dtype, 0), vcache=(kcache if vcache is None else vcache, kcache.dtype, 0),
-            seq_start=(seq_start, I32, B), path=(path, I32, 0), count=(count, I32, 0))
-    _here("cache_compact", [block_table])
-    f = fn("draft", "lumen_cache_compact", [P, P, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                            c_int, c_int, P])
+    dtype = kcache.dtype
+    _arrays("cache_compact", ("kcache", kcache, dtype, 0), ("vcache", kcache if vcache is None else vcache, dtype, 0),
+            ("seq_start", seq_start, I32, B), ("path", path, I32, 0), ("count", count, I32, 0))
+    _here("cache_compact", block_table)
+    f = fn("draft", "lumen_cache_compact", _CACHE_COMPACT_ARGS)
     check(f(ptr(kcache), ptr(vcache), ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(seq_start), ptr(path),
             path.shape[1], ptr(count), B, layers, n_pages, nkv, d, dv, int(layout), int(v_layout), 4 if kcache.dtype == F32 else 2,
             stream_ptr()), "cache_compact")

@@ -37,6 +37,7 @@ FUSED_DECODE_ROWS = (4, 16)
 @register_part("mixer", "gqa_attention")
 class GQAttention:
     graph_safe = True
+    tree_safe = True
 
     @classmethod
     def tensors(cls, spec):
@@ -132,7 +133,7 @@ class GQAttention:
 
 def causal_attention(q, kc, vc, table, ctx, k_layout, v_layout, window, scale, chunk=0, softcap=0.0,
                      sink=False, gate=None, gate_col=0, head_gate=False, keep_first=0, key_dim=None, value_dim=None):
-    """Chooses the kernel by the step's shape: the split-KV kernel when every sequence
+    """Chooses the kernel by the step's shape: the tree kernel for trees of drafted tokens, the split-KV kernel when every sequence
     brings one token, the flash kernel for prompts, and the general kernel for the
     32-bit path and for head sizes the fast kernels do not take. All agree within rounding.
     q [N, nq, d], as wide as the cache's keys; key_dim and value_dim say how much of keys and values is
@@ -140,6 +141,13 @@ def causal_attention(q, kc, vc, table, ctx, k_layout, v_layout, window, scale, c
     options of ops.kernels.attn_generic_opt."""
     nq, d = q.shape[1], q.shape[2]
     nkv, dv = kc.shape[1], vc.shape[3]
+    if ctx.tree_mask is not None and not ctx.is_decode:
+        # trees of drafted tokens (a sequence that brings one token has the tree of a decode step); parts that need
+        # the other options are not `tree_safe`
+        if chunk or gate is not None or keep_first or value_dim or key_dim not in (None, d):
+            raise ValueError("tree attention takes a window, capped scores and a sink, no other option")
+        return K.attn_tree(q, kc, vc, table, ctx.cu_q, ctx.seq_start, ctx.tok_seq, ctx.rope_pos, ctx.tree_mask, window, scale,
+                           layout=k_layout, v_layout=v_layout, softcap=softcap, sink=sink)
     opts = dict(chunk=chunk, softcap=softcap, sink=sink, gate=gate, gate_col=gate_col, head_gate=head_gate,
                 keep_first=keep_first, value_dim=value_dim)
     fast = (k_layout == K.LAYOUT_SW128 and v_layout == K.LAYOUT_SW128 and q.dtype == torch.bfloat16
@@ -237,6 +245,10 @@ class WideNormAttention:
         self.q_norm, self.k_norm = f32(f"{pre}.q.norm"), f32(f"{pre}.k.norm")
         self.sink = f32(f"{pre}.sink") if p.get("sink", False) else None
         self.o = Linear(weights[f"{pre}.o"], runtime)
+
+    @property
+    def tree_safe(self):
+        return not self.taps and not self.gated
 
     def cache_need(self):
         return CacheNeed(self.G, self.d, self.window, v_dim=0 if self.dv == self.d else self.dv)
@@ -357,6 +369,11 @@ class HeadNormAttention:
             self.q_norm, self.k_norm = f32(f"{pre}.q.norm"), f32(f"{pre}.k.norm")
         self.gate_col = self.H * self.d + self.G * (self.d + self.dv)
         self.o = Linear(weights[f"{pre}.o"], runtime)
+
+    @property
+    def tree_safe(self):
+        padded = self.padded and self.runtime.dtype == torch.bfloat16 and (self.d % 64 or self.dv % 64)
+        return not (self.chunk or self.gated or self.keep_first or padded)
 
     def cache_need(self):
         return CacheNeed(self.G, self.d, self.window, v_dim=0 if self.dv == self.d else self.dv, chunk=self.chunk,

@@ -150,3 +150,71 @@ def test_segments_of_partial_results_fit_their_room():
         seg = min(np_, max(4, (q * G + 7) // 8))
         nseg = min(-(-np_ // seg), 64)
         assert nseg == 1 or (width > 4 and q * nseg <= q + -(-8 * width // G))
+
+
+def drafting_engine(**over):
+    """An Engine's bookkeeping without a device: enough for what verify refuses."""
+    from lumenllm_b200.cache import CacheNeed, KVCache
+    from lumenllm_b200.engine import Engine
+    e = Engine.__new__(Engine)
+    e.cache = KVCache({0: CacheNeed(1, 16)}, 640, 4, max_positions=512)
+    e.model = type("M", (), {"tree_safe": True})()
+    e.vocab_size, e.max_seq_len, e.max_step_tokens = 100, 300, 400
+    for k, v in over.items():
+        setattr(e, k, v)
+    return e
+
+
+@pytest.mark.parametrize("drafts,kw,says", [
+    ([], {}, "at least one sequence"),
+    ([(0, [1], [-1]), (0, [1], [-1])], {}, "twice"),
+    ([(3, [1], [-1])], {}, "not live"),
+    ([(0, [], [])], {}, "at least one token"),
+    ([(0, [1, 100], [-1, 0])], {}, "vocabulary"),
+    ([(0, [1] * 257, [-1] + [0] * 256)], {}, "up to 256"),
+    ([(0, [1, 2], [-1])], {}, "parents"),
+    ([(0, [1, 2], [0, 0])], {}, "parents"),
+    ([(0, [1, 2], [-1, 1])], {}, "parents"),
+    ([(0, [1, 2], [-1, -1])], {}, "parents"),
+    ([(0, [1] * 250, [-1] + [0] * 249), (1, [1] * 200, [-1] + [0] * 199)], {}, "exceed a step"),
+    ([(0, [1], [-1])], dict(configs=[]), "one sampling config"),
+    ([(0, [1, 2], [-1, 0])], dict(configs=["hot"]), "uniform numbers"),
+    ([(0, [1, 2], [-1, 0])], dict(configs=["hot"], uniforms=[[0.5]]), "2 tokens deep"),
+    ([(0, [1, 2], [-1, 0])], dict(configs=["cold"], uniforms=[[0.5], [0.5]]), "one row of uniform numbers"),
+])
+def test_verify_refuses(drafts, kw, says):
+    from lumenllm_b200 import DraftEntry, SamplingConfig, StepError
+    e = drafting_engine()
+    assert [e.cache.alloc_slot() for _ in range(2)] == [0, 1]
+    named = {"hot": SamplingConfig(temperature=0.7), "cold": SamplingConfig()}
+    kw = {k: [named.get(x, x) if isinstance(x, str) else x for x in v] for k, v in kw.items()}
+    with pytest.raises(StepError, match=says):
+        e._validate_drafts([DraftEntry(*d) for d in drafts], kw.get("configs"), kw.get("uniforms"))
+    assert e.cache.length(0) == 0 and e.cache.free_tokens() == 640        # nothing was taken
+
+
+def test_verify_refuses_models_and_long_sequences():
+    from lumenllm_b200 import DraftEntry, StepError
+    e = drafting_engine()
+    e.cache.alloc_slot()
+    e.cache.commit(0, 298)
+    with pytest.raises(StepError, match="context"):
+        e._validate_drafts([DraftEntry(0, [1, 2, 3], [-1, 0, 0])], None, None)
+    assert e._validate_drafts([DraftEntry(0, [1, 2], [-1, 0])], None, None) == [[0, 1]]
+    e.model.tree_safe = False
+    with pytest.raises(StepError, match="no drafts"):
+        e._validate_drafts([DraftEntry(0, [1], [-1])], None, None)
+
+
+def test_which_mixers_take_trees():
+    from lumenllm_b200.parts import attention as A
+    assert A.GQAttention.tree_safe
+    safe = lambda cls, **kw: cls.tree_safe.fget(type("X", (), kw)())
+    assert safe(A.WideNormAttention, taps=0, gated=False)
+    assert not safe(A.WideNormAttention, taps=4, gated=False) and not safe(A.WideNormAttention, taps=0, gated=True)
+    run = type("R", (), {"dtype": BF16})()
+    base = dict(chunk=0, gated=False, keep_first=0, padded=False, runtime=run, d=96, dv=64)
+    assert safe(A.HeadNormAttention, **base)
+    for over in (dict(chunk=64), dict(gated=True), dict(keep_first=4), dict(padded=True)):
+        assert not safe(A.HeadNormAttention, **{**base, **over})
+    assert safe(A.HeadNormAttention, **{**base, "padded": True, "d": 128})
