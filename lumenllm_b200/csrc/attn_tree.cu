@@ -10,14 +10,18 @@
 // the tensor-core kernel of attn_tree_tc.cu.
 //
 // General kernel: a block has 32 rows (node, query head) of one kv head and a segment of the keys, and takes a page (64 keys)
-// at a time through shared memory in float32, keys and then values in the same place: scores by register tiles of 4 x 4, the
-// softmax with a running maximum and sum, values by tiles of 8 rows x 4 columns a thread. It is bound by the FMA pipe where
-// a step has 32 rows a kv head and by the copies through registers where it has few.
+// at a time through shared memory in float32: scores by register tiles of 4 rows x 4 keys (the two float32 products of one instruction
+// are neighbouring numbers of a key), the softmax with a running maximum and sum, values by tiles of 8 rows x 4 columns a thread (two
+// rows an instruction). It is bound by the FMA pipe where a step has 32 rows a kv head. Float32 tiles are asked for ahead, by
+// asynchronous copies: keys under the products of the values before them and the other way round; bfloat16 tiles are
+// converted on the way, and tiles that do not fit twice are taken one behind the other.
+#include "tmem_attn.cuh"
 #include "tree_plan.cuh"
 
 #define TA_THREADS 128
 #define TA_ROWS 32
 #define TA_PROW 36                // numbers a key's row of weights takes in shared memory
+#define TA_LOADS 8                // 16-byte loads that a thread has under way
 
 struct TreeArgs {
     const void* q;
@@ -44,46 +48,68 @@ __device__ __forceinline__ float ta_close(float m, float l, const float* sink, i
     return f / (l * f + expf(s - top));
 }
 
-// A page tile of `cols` numbers a row, into rows of `stride` float32 (columns up to `pad` zero); rows from `valid` on are zero.
-// Returns whether a number that is not finite was among this thread's.
+// A page tile of `cols` numbers a row into rows of `stride` float32: whole numbers up to `pad` columns (zeros behind cols); rows from
+// `valid` on are zeros.
 template <typename T>
-__device__ __forceinline__ bool ta_stage(float* dst, int stride, int pad, const T* tile, int cols, int layout, int valid, int vec) {
-    bool bad = false;
+__device__ __forceinline__ void ta_stage(float* dst, int stride, int pad, const T* tile, int cols, int layout, int valid, bool vec) {
     if (vec) {
         constexpr int E = 16 / (int)sizeof(T);
-        const int pieces = cols / E, padded = pad / E;
-        for (int idx = threadIdx.x; idx < LUMEN_PAGE * padded; idx += TA_THREADS) {
-            const int r = idx / padded, c = idx - r * padded;
-            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-            if (r < valid && c < pieces) raw = *reinterpret_cast<const uint4*>(tile + tile_offset(layout, r, c * E, cols));
-            const T* x = reinterpret_cast<const T*>(&raw);
-            float f[E];
+        const int pieces = cols / E, all = LUMEN_PAGE * pieces;
+        const int step_r = TA_THREADS / pieces, step_c = TA_THREADS - step_r * pieces;
+        int r = threadIdx.x / pieces, c = threadIdx.x - r * pieces;
+        for (int base = threadIdx.x; base < all; base += TA_LOADS * TA_THREADS) {
+            uint4 raw[TA_LOADS];
+            int at[TA_LOADS];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                f[i] = to_f32(x[i]);
-                bad |= !(fabsf(f[i]) <= 3.402823466e38f);
+            for (int i = 0; i < TA_LOADS; ++i) {
+                raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                at[i] = r * stride + c * E;
+                if (r < valid) raw[i] = *reinterpret_cast<const uint4*>(tile + tile_offset(layout, r, c * E, cols));
+                r += step_r;
+                c += step_c;
+                if (c >= pieces) { c -= pieces; ++r; }
             }
 #pragma unroll
-            for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(dst + r * stride + c * E + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            for (int i = 0; i < TA_LOADS; ++i) {
+                if (base + i * TA_THREADS >= all) break;
+                const T* x = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+                for (int e = 0; e < E; e += 4)
+                    *reinterpret_cast<float4*>(dst + at[i] + e) = make_float4(to_f32(x[e]), to_f32(x[e + 1]), to_f32(x[e + 2]), to_f32(x[e + 3]));
+            }
         }
     } else {
         for (int idx = threadIdx.x; idx < LUMEN_PAGE * pad; idx += TA_THREADS) {
             const int r = idx / pad, e = idx - r * pad;
-            const float f = (r < valid && e < cols) ? to_f32(tile[tile_offset(layout, r, e, cols)]) : 0.0f;
-            bad |= !(fabsf(f) <= 3.402823466e38f);
-            dst[r * stride + e] = f;
+            dst[r * stride + e] = (r < valid && e < cols) ? to_f32(tile[tile_offset(layout, r, e, cols)]) : 0.0f;
         }
     }
-    return bad;
+}
+// The same for float32 rows of whole 16 bytes, without waiting for them.
+__device__ __forceinline__ void ta_stage_async(float* dst, int stride, const float* tile, int cols, int valid) {
+    const int pieces = cols >> 2, step_r = TA_THREADS / pieces, step_c = TA_THREADS - step_r * pieces;
+    int r = threadIdx.x / pieces, c = threadIdx.x - r * pieces;
+    for (int idx = threadIdx.x; idx < LUMEN_PAGE * pieces; idx += TA_THREADS) {
+        const int bytes = r < valid ? 16 : 0;           // 0: zeros, nothing is read
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * stride + 4 * c)),
+                     "l"(tile + (r < valid ? r * cols + 4 * c : 0)), "r"(bytes)
+                     : "memory");
+        r += step_r;
+        c += step_c;
+        if (c >= pieces) { c -= pieces; ++r; }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-template <typename T, int NC>
+// ASYNC: keys and values have places of their own, and copies run ahead (float32 in rows of whole 16 bytes).
+template <typename T, int NC, bool ASYNC>
 __global__ void __launch_bounds__(TA_THREADS)
 attn_tree_kernel(const TreeArgs a) {
     pdl_wait();      // nothing of this kernel touches global memory before this
     pdl_trigger();
     extern __shared__ __align__(16) float ta_smem[];
-    __shared__ float s_corr[TA_ROWS], s_inv[TA_ROWS];
+    __shared__ __align__(16) float s_corr[TA_ROWS];
+    __shared__ float s_inv[TA_ROWS];
     __shared__ int s_unit[2];
     const int G = a.nq / a.nkv, tid = threadIdx.x;
     const int kvh = blockIdx.x % a.nkv, seg = blockIdx.y;
@@ -100,14 +126,49 @@ attn_tree_kernel(const TreeArgs a) {
     if (seg >= plan.nseg) return;
     const int f0 = s_unit[1] * TA_ROWS, nrows = min(TA_ROWS, sq.q * G - f0);
     const int dp = (a.d + 3) & ~3, ks = dp + 4;
+    constexpr int VS = 128 * NC;
     float* qs = ta_smem;                          // [32][ks]
-    float* kv = qs + TA_ROWS * ks;                // [64][ks] keys, then [64][128 NC] values
-    float* ps = kv + LUMEN_PAGE * max(ks, 128 * NC);      // [64][TA_PROW]: weights, a key's rows together
+    float* keys = qs + TA_ROWS * ks;              // [64][ks]
+    float* vals = ASYNC ? keys + LUMEN_PAGE * ks : keys;      // [64][VS]
+    float* ps = ASYNC ? vals + LUMEN_PAGE * VS : keys + LUMEN_PAGE * max(ks, VS);      // [64][TA_PROW]: weights, a key's rows together
     const T* q = (const T*)a.q;
-
-    for (int idx = tid; idx < TA_ROWS * dp; idx += TA_THREADS) {
-        const int r = idx / dp, e = idx - r * dp, f = f0 + r;
-        qs[r * ks + e] = (r < nrows && e < a.d) ? to_f32(q[((size_t)(sq.n0 + f / G) * a.nq + kvh * G + f % G) * a.d + e]) : 0.0f;
+    const int* bt = a.block_table + (size_t)b * a.bt_stride;
+    const int pg0 = plan.first(seg), npages = plan.count(seg);
+    auto tile_of = [&](int i) {
+        const int page = bt[pg0 + i];
+        return ((size_t)((unsigned)page < (unsigned)a.n_pages ? page : 0) * a.nkv + kvh) * (size_t)LUMEN_PAGE;
+    };
+    auto valid_of = [&](int i) { return min(LUMEN_PAGE, sq.end - (pg0 + i) * LUMEN_PAGE); };
+    if (ASYNC) {
+        const size_t tile = tile_of(0);
+        ta_stage_async(keys, ks, (const float*)a.kcache + tile * a.d, a.d, valid_of(0));
+        ta_stage_async(vals, VS, (const float*)a.vcache + tile * a.dv, a.dv, valid_of(0));
+    }
+    {
+        // Q: four threads a row
+        const int r = tid >> 2, f = f0 + min(r, nrows - 1);
+        const T* src = q + ((size_t)(sq.n0 + f / G) * a.nq + kvh * G + f % G) * a.d;
+        float* dst = qs + r * ks;
+        if (a.vec & 4) {
+            constexpr int E = 16 / (int)sizeof(T);
+            const int pieces = r < nrows ? a.d / E : 0;
+            for (int c0 = tid & 3; c0 < pieces; c0 += 4 * TA_LOADS) {
+                uint4 raw[TA_LOADS];
+#pragma unroll
+                for (int i = 0; i < TA_LOADS; ++i)
+                    if (c0 + 4 * i < pieces) raw[i] = *reinterpret_cast<const uint4*>(src + (c0 + 4 * i) * E);
+#pragma unroll
+                for (int i = 0; i < TA_LOADS; ++i) {
+                    if (c0 + 4 * i >= pieces) break;
+                    const T* x = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+                    for (int e = 0; e < E; e += 4)
+                        *reinterpret_cast<float4*>(dst + (c0 + 4 * i) * E + e) = make_float4(to_f32(x[e]), to_f32(x[e + 1]), to_f32(x[e + 2]), to_f32(x[e + 3]));
+                }
+            }
+        }
+        for (int e = tid & 3; e < dp; e += 4)           // rows that there are not, columns behind the last
+            if (r >= nrows || !(a.vec & 4)) dst[e] = r < nrows && e < a.d ? to_f32(src[e]) : 0.0f;
     }
     // scores: rows 4 rg .. 4 rg + 3, keys kg, kg + 16, kg + 32, kg + 48
     const int rg = tid >> 4, kg = tid & 15;
@@ -120,113 +181,134 @@ attn_tree_kernel(const TreeArgs a) {
         pos[i] = max(a.tok_pos[n], sq.start);
     }
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    // values: rows 8 wr .. 8 wr + 7, columns 4 lane + 128 c .. + 3
+    // values: rows 8 wr .. 8 wr + 7 in pairs, columns 4 lane + 128 c .. + 3
     const int wr = tid >> 5, lane = tid & 31;
-    float acc[8][4 * NC];
+    pt_f2 acc[4][4 * NC];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < 4 * NC; ++c) acc[r][c] = 0.0f;
-    const int* bt = a.block_table + (size_t)b * a.bt_stride;
+        for (int c = 0; c < 4 * NC; ++c) acc[r][c] = 0ull;
 
-    for (int pg = plan.first(seg), last = pg + plan.count(seg); pg < last; ++pg) {
-        int page = bt[pg];
-        if ((unsigned)page >= (unsigned)a.n_pages) page = 0;
-        const size_t tile = (size_t)page * a.nkv + kvh;
-        const int jb = pg * LUMEN_PAGE, valid = min(LUMEN_PAGE, sq.end - jb);
-        __syncthreads();
-        ta_stage<T>(kv, ks, dp, (const T*)a.kcache + tile * (size_t)(LUMEN_PAGE * a.d), a.d, a.layout, valid, a.vec & 1);
-        __syncthreads();
-        float s[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[i][k] = 0.0f;
-        for (int e = 0; e < dp; e += 4) {
-            float4 x[4], y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(qs + (4 * rg + i) * ks + e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const float4*>(kv + (kg + 16 * k) * ks + e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    s[i][k] = fmaf(x[i].x, y[k].x, s[i][k]);
-                    s[i][k] = fmaf(x[i].y, y[k].y, s[i][k]);
-                    s[i][k] = fmaf(x[i].z, y[k].z, s[i][k]);
-                    s[i][k] = fmaf(x[i].w, y[k].w, s[i][k]);
-                }
+    for (int i = 0; i < npages; ++i) {
+        const int jb = (pg0 + i) * LUMEN_PAGE, valid = valid_of(i);
+        const size_t tile = tile_of(i);
+        if (ASYNC) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");        // the keys; the values may still be under way
+        } else {
+            __syncthreads();                      // the values before have been read
+            ta_stage<T>(keys, ks, dp, (const T*)a.kcache + tile * a.d, a.d, a.layout, valid, a.vec & 1);
         }
-        float corr[4];
+        __syncthreads();
+        pt_f2 s2[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned long long seen = tree_seen(jb, sq, mask[i], a.W, pos[i], a.window, a.tok_pos + sq.n0);
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s2[x][k] = 0ull;
+#pragma unroll 2
+        for (int e = 0; e < dp; e += 4) {
+            ulonglong2 x[4], y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(qs + (4 * rg + r) * ks + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const ulonglong2*>(keys + (kg + 16 * k) * ks + e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s2[r][k] = pt_fma2(x[r].y, y[k].y, pt_fma2(x[r].x, y[k].x, s2[r][k]));
+        }
+        float s[4][4], corr[4];
+        const bool all = jb + LUMEN_PAGE <= sq.start && a.window == 0;       // every row sees the whole page
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned long long seen = all ? ~0ull : tree_seen(jb, sq, mask[r], a.W, pos[r], a.window, a.tok_pos + sq.n0);
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float x = s[i][k] * a.scale;
+                float even, odd;
+                pt_unpair(s2[r][k], even, odd);
+                float x = (even + odd) * a.scale;
                 if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-                s[i][k] = (seen >> (kg + 16 * k)) & 1 ? x : -INFINITY;
-                top = fmaxf(top, s[i][k]);
+                s[r][k] = (seen >> (kg + 16 * k)) & 1 ? x : -INFINITY;
+                top = fmaxf(top, s[r][k]);
             }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float mn = fmaxf(m[i], top), base = mn == -INFINITY ? 0.0f : mn;
-            corr[i] = m[i] == -INFINITY ? 0.0f : expf(m[i] - mn);
+            const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
+            corr[r] = m[r] == -INFINITY ? 0.0f : expf(m[r] - mn);
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                s[i][k] = expf(s[i][k] - base);      // 0 for a masked key, also where none has been seen yet
-                sum += s[i][k];
+                s[r][k] = expf(s[r][k] - base);      // 0 for a masked key, also where none has been seen yet
+                sum += s[r][k];
             }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[i] = l[i] * corr[i] + sum;
-            m[i] = mn;
+            l[r] = l[r] * corr[r] + sum;
+            m[r] = mn;
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             *reinterpret_cast<float4*>(ps + (kg + 16 * k) * TA_PROW + 4 * rg) = make_float4(s[0][k], s[1][k], s[2][k], s[3][k]);
-        if (kg == 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s_corr[4 * rg + i] = corr[i];
+        if (kg == 0) *reinterpret_cast<float4*>(s_corr + 4 * rg) = make_float4(corr[0], corr[1], corr[2], corr[3]);
         __syncthreads();                          // the keys have been read, the weights are there
-        const bool bad = ta_stage<T>(kv, 128 * NC, 128 * NC, (const T*)a.vcache + tile * (size_t)(LUMEN_PAGE * a.dv), a.dv, a.v_layout,
-                                     valid, a.vec & 2);
-        const bool any_bad = __syncthreads_or(bad);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const float c = s_corr[8 * wr + r];
-#pragma unroll
-            for (int x = 0; x < 4 * NC; ++x) acc[r][x] *= c;
+        if (ASYNC) {
+            if (i + 1 < npages) ta_stage_async(keys, ks, (const float*)a.kcache + tile_of(i + 1) * a.d, a.d, valid_of(i + 1));
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");        // the values
+        } else {
+            ta_stage<T>(vals, VS, VS, (const T*)a.vcache + tile * a.dv, a.dv, a.v_layout, valid, a.vec & 2);
         }
+        __syncthreads();
+        bool any_bad = false;
+        if (!all) {
+            // a value that is no number, on a page that some row does not see whole
+            bool bad = false;
+            for (int r = wr; r < valid; r += TA_THREADS / 32)
+                for (int e = lane; e < a.dv; e += 32) bad |= !(fabsf(vals[r * VS + e]) <= 3.402823466e38f);
+            any_bad = __syncthreads_or(bad);
+        }
+        {
+            const ulonglong2 c01 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * wr), c23 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * wr + 4);
+            const pt_f2 c[4] = {c01.x, c01.y, c23.x, c23.y};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int x = 0; x < 4 * NC; ++x) acc[r][x] = pt_fma2(acc[r][x], c[r], 0ull);
+        }
+#pragma unroll 2
         for (int k = 0; k < valid; ++k) {
-            float w[8];
-            *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(ps + k * TA_PROW + 8 * wr);
-            *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(ps + k * TA_PROW + 8 * wr + 4);
+            const ulonglong2 w01 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * wr);
+            const ulonglong2 w23 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * wr + 4);
+            const pt_f2 w[4] = {w01.x, w01.y, w23.x, w23.y};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const float4 v = *reinterpret_cast<const float4*>(kv + k * (128 * NC) + 128 * c + 4 * lane);
+                const float4 v = *reinterpret_cast<const float4*>(vals + k * VS + 128 * c + 4 * lane);
+                const pt_f2 vv[4] = {pt_pair(v.x, v.x), pt_pair(v.y, v.y), pt_pair(v.z, v.z), pt_pair(v.w, v.w)};
                 if (any_bad) {                    // nothing of a masked value, not even 0 times infinity
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (w[r] != 0.0f) {
-                            acc[r][4 * c] = fmaf(w[r], v.x, acc[r][4 * c]);
-                            acc[r][4 * c + 1] = fmaf(w[r], v.y, acc[r][4 * c + 1]);
-                            acc[r][4 * c + 2] = fmaf(w[r], v.z, acc[r][4 * c + 2]);
-                            acc[r][4 * c + 3] = fmaf(w[r], v.w, acc[r][4 * c + 3]);
+                    for (int r = 0; r < 4; ++r) {
+                        float w0, w1;
+                        pt_unpair(w[r], w0, w1);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            float a0, a1, p0, p1;
+                            pt_unpair(acc[r][4 * c + x], a0, a1);
+                            pt_unpair(pt_fma2(w[r], vv[x], acc[r][4 * c + x]), p0, p1);
+                            acc[r][4 * c + x] = pt_pair(w0 != 0.0f ? p0 : a0, w1 != 0.0f ? p1 : a1);
                         }
+                    }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        acc[r][4 * c] = fmaf(w[r], v.x, acc[r][4 * c]);
-                        acc[r][4 * c + 1] = fmaf(w[r], v.y, acc[r][4 * c + 1]);
-                        acc[r][4 * c + 2] = fmaf(w[r], v.z, acc[r][4 * c + 2]);
-                        acc[r][4 * c + 3] = fmaf(w[r], v.w, acc[r][4 * c + 3]);
-                    }
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[r][4 * c + x] = pt_fma2(w[r], vv[x], acc[r][4 * c + x]);
                 }
             }
+        }
+        if (ASYNC) {
+            __syncthreads();                      // the values have been read
+            if (i + 1 < npages) ta_stage_async(vals, VS, (const float*)a.vcache + tile_of(i + 1) * a.dv, a.dv, valid_of(i + 1));
+            else asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
     const bool whole = plan.nseg == 1;
@@ -247,21 +329,29 @@ attn_tree_kernel(const TreeArgs a) {
         const int row = 8 * wr + r, f = f0 + row;
         if (row >= nrows) continue;
         const int head = kvh * G + f % G;
-        if (whole) {
-            T* dst = (T*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv;
-            const float inv = s_inv[row];
+        const float inv = whole ? s_inv[row] : 1.0f;
+        T* dst = (T*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv;
+        float* part = a.part_o + ((pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head) * (long long)a.dv;
 #pragma unroll
-            for (int c = 0; c < 4 * NC; ++c) {
-                const int e = 4 * lane + 128 * (c >> 2) + (c & 3);
-                if (e < a.dv) dst[e] = from_f32<T>(acc[r][c] * inv);
-            }
-        } else {
-            float* dst = a.part_o + ((pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head) * (long long)a.dv;
+        for (int c = 0; c < NC; ++c) {
+            const int e = 4 * lane + 128 * c;
+            float v[4];
 #pragma unroll
-            for (int c = 0; c < 4 * NC; ++c) {
-                const int e = 4 * lane + 128 * (c >> 2) + (c & 3);
-                if (e < a.dv) dst[e] = acc[r][c];
+            for (int x = 0; x < 4; ++x) {
+                float even, odd;
+                pt_unpair(acc[r >> 1][4 * c + x], even, odd);
+                v[x] = (r & 1 ? odd : even) * inv;
             }
+            if (!whole && (a.dv & 3) == 0) {
+                if (e < a.dv) *reinterpret_cast<float4*>(part + e) = make_float4(v[0], v[1], v[2], v[3]);
+                continue;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (e + x < a.dv) {
+                    if (whole) dst[e + x] = from_f32<T>(v[x]);
+                    else part[e + x] = v[x];
+                }
         }
     }
 }
@@ -342,17 +432,22 @@ attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
         if (e + i < a.dv) dst[i] = from_f32<T>(v[i]);
 }
 
-template <typename T, int NC>
-static cudaError_t ta_go(const TreeArgs& a, const int* tok_seq, int max_segs, cudaStream_t stream) {
-    const int ks = ((a.d + 3) & ~3) + 4, wide = ks > 128 * NC ? ks : 128 * NC;
-    const int smem = (TA_ROWS * ks + LUMEN_PAGE * wide + LUMEN_PAGE * TA_PROW) * (int)sizeof(float);
-    auto k = attn_tree_kernel<T, NC>;
+template <typename T, int NC, bool ASYNC>
+static cudaError_t ta_run(const TreeArgs& a, const int* tok_seq, int smem, int max_segs, cudaStream_t stream) {
+    auto k = attn_tree_kernel<T, NC, ASYNC>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)a.N * (a.nq / a.nkv) / TA_ROWS + a.B;
     e = lumen_launch(k, dim3((unsigned)(tiles * a.nkv), max_segs), dim3(TA_THREADS), smem, stream, a);
     if (e != cudaSuccess || max_segs == 1) return e;
     return lumen_launch(attn_tree_join_kernel<T>, dim3(a.N, ((a.dv + 3) / 4 * a.nq + 127) / 128), dim3(128), 0, stream, a, tok_seq);
+}
+template <typename T, int NC>
+static cudaError_t ta_go(const TreeArgs& a, const int* tok_seq, int max_segs, cudaStream_t stream) {
+    const int ks = ((a.d + 3) & ~3) + 4, vs = 128 * NC, fixed = TA_ROWS * ks + LUMEN_PAGE * TA_PROW;
+    const int both = (fixed + LUMEN_PAGE * (ks + vs)) * (int)sizeof(float), one = (fixed + LUMEN_PAGE * (ks > vs ? ks : vs)) * (int)sizeof(float);
+    if (sizeof(T) == 4 && NC < 4 && (a.vec & 3) == 3 && both <= 226 * 1024) return ta_run<T, NC, sizeof(T) == 4 && NC < 4>(a, tok_seq, both, max_segs, stream);
+    return ta_run<T, NC, false>(a, tok_seq, one, max_segs, stream);
 }
 
 #include "attn_tree_tc.cuh"
@@ -397,7 +492,8 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     if ((tc && (!tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale) || !tt_aligned(q, kcache, vcache, out))) || scratch_k < need ||
         (need && !scratch) || ((uintptr_t)scratch & 31))
         return LUMEN_ERR_BAD_ARGUMENT;
-    const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0);
+    const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0) |
+                    (((uintptr_t)q & 15) == 0 && d * es % 16 == 0 ? 4 : 0);
     // the maxima and sums first: the rows behind them lie on 16 bytes where dv is a multiple of 4
     const long long pairs = ((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2;
     const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out,

@@ -8,7 +8,7 @@
 
 #define TREE_MAX_NODES 256        // nodes of a sequence that the masks and the walk cover
 #define TREE_MAX_SEGS 64          // a sequence is never cut into more segments than this
-#define TREE_MIN_SEG 4            // pages of the shortest segment
+#define TREE_MIN_SEG 2            // pages of the shortest segment
 
 struct TreeSeq {
     int n0, q;        // its first token of the step, its nodes
@@ -34,7 +34,7 @@ __device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg
 }
 // The general kernel's cut of them: nseg segments of per or per + 1 pages (the first rem have one more).
 // A segment's partial result is rows x dv float32, its keys and values are pages x 64 x (d + dv) numbers: with a page for
-// eight rows at least, partials come to an eighth (bfloat16) or a sixteenth of what the segment reads. The cut depends on the
+// sixteen rows at least, partials come to an eighth (float32) or a quarter of what the segment reads. The cut depends on the
 // sequence alone, never on its neighbours in the batch or the page table's width.
 struct TreePlan {
     int pg_lo, np, nseg, per, rem;
@@ -45,15 +45,15 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int 
     TreePlan p;
     tree_pages(s, window, p.pg_lo, p.np);
     const long long rows = (long long)s.q * G;
-    const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 7) / 8));
+    const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 15) / 16));
     p.nseg = min((p.np + seg - 1) / seg, TREE_MAX_SEGS);
     p.per = p.np / p.nseg;
     p.rem = p.np - p.per * p.nseg;
     return p;
 }
 // Partial results of sequence b lie from this (token, segment) pair on, node i's segments at i * nseg: q * nseg is at most
-// q + 8 width / G whatever the lengths are.
-__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return (8LL * width + G - 1) / G; }
+// q + 16 width / G whatever the lengths are.
+__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return (16LL * width + G - 1) / G; }
 __device__ __forceinline__ long long tree_part_base(int b, int n0, int width, int G) {
     return (long long)b * tree_part_room(width, G) + n0;
 }
