@@ -11,8 +11,10 @@
 //
 // General kernel: a block has 32 rows (node, query head) of one kv head and a segment of the keys, and takes a page (64 keys)
 // at a time through shared memory in float32: scores by register tiles of 4 rows x 4 keys (the two float32 products of one instruction
-// are neighbouring numbers of a key), the softmax with a running maximum and sum, values by tiles of 8 rows x 4 columns a thread (two
-// rows an instruction). It is bound by the FMA pipe where a step has 32 rows a kv head. Float32 tiles are asked for ahead, by
+// are neighbouring numbers of a key), the softmax with a running maximum and sum, values by tiles of 8 rows x 8 columns a thread (two
+// rows an instruction), the even keys by one half of the block, the odd ones by the other. What bounds it is what shared memory
+// hands to registers, 128 bytes a cycle: a tile's side is what counts, and reads that all lanes share cost as much as others (scores of 8
+// rows x 2 keys a lane, a warp's rows read by all its lanes, took longer). Float32 tiles are asked for ahead, by
 // asynchronous copies: keys under the products of the values before them and the other way round; bfloat16 tiles are
 // converted on the way, and tiles that do not fit twice are taken one behind the other.
 #include "tmem_attn.cuh"
@@ -109,9 +111,9 @@ attn_tree_kernel(const TreeArgs a) {
     pdl_trigger();
     extern __shared__ __align__(16) float ta_smem[];
     __shared__ __align__(16) float s_corr[TA_ROWS];
-    __shared__ float s_inv[TA_ROWS];
-    __shared__ int s_unit[2];
-    const int G = a.nq / a.nkv, tid = threadIdx.x;
+    __shared__ int s_unit[2], s_tok[TA_ROWS], s_head[TA_ROWS];
+    __shared__ float2 s_ml[TA_ROWS];
+    const int G = a.nq / a.nkv, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.x % a.nkv, seg = blockIdx.y;
     if (tid < 32) {
         int b, tile;
@@ -128,9 +130,9 @@ attn_tree_kernel(const TreeArgs a) {
     const int dp = (a.d + 3) & ~3, ks = dp + 4;
     constexpr int VS = 128 * NC;
     float* qs = ta_smem;                          // [32][ks]
-    float* keys = qs + TA_ROWS * ks;              // [64][ks]
+    float* ps = qs + TA_ROWS * ks;                // [64][TA_PROW]: weights, a key's rows together
+    float* keys = ps + LUMEN_PAGE * TA_PROW;      // [64][ks]
     float* vals = ASYNC ? keys + LUMEN_PAGE * ks : keys;      // [64][VS]
-    float* ps = ASYNC ? vals + LUMEN_PAGE * VS : keys + LUMEN_PAGE * max(ks, VS);      // [64][TA_PROW]: weights, a key's rows together
     const T* q = (const T*)a.q;
     const int* bt = a.block_table + (size_t)b * a.bt_stride;
     const int pg0 = plan.first(seg), npages = plan.count(seg);
@@ -146,8 +148,9 @@ attn_tree_kernel(const TreeArgs a) {
     }
     {
         // Q: four threads a row
-        const int r = tid >> 2, f = f0 + min(r, nrows - 1);
-        const T* src = q + ((size_t)(sq.n0 + f / G) * a.nq + kvh * G + f % G) * a.d;
+        const int r = tid >> 2, f = f0 + min(r, nrows - 1), node = f / G, head = kvh * G + f - node * G;
+        if ((tid & 3) == 0) { s_tok[r] = sq.n0 + node; s_head[r] = head; }
+        const T* src = q + ((size_t)(sq.n0 + node) * a.nq + head) * a.d;
         float* dst = qs + r * ks;
         if (a.vec & 4) {
             constexpr int E = 16 / (int)sizeof(T);
@@ -167,27 +170,33 @@ attn_tree_kernel(const TreeArgs a) {
                 }
             }
         }
-        for (int e = tid & 3; e < dp; e += 4)           // rows that there are not, columns behind the last
-            if (r >= nrows || !(a.vec & 4)) dst[e] = r < nrows && e < a.d ? to_f32(src[e]) : 0.0f;
+        if (r >= nrows || !(a.vec & 4))                  // rows that there are not, columns behind the last
+            for (int e = tid & 3; e < dp; e += 4) dst[e] = r < nrows && e < a.d ? to_f32(src[e]) : 0.0f;
     }
-    // scores: rows 4 rg .. 4 rg + 3, keys kg, kg + 16, kg + 32, kg + 48
+    __syncthreads();
+    // scores: rows 4 rg .. 4 rg + 3, keys kg, kg + 16, kg + 32, kg + 48 (a warp that has no rows there sits out)
     const int rg = tid >> 4, kg = tid & 15;
+    const bool idle = 8 * warp >= nrows;
     const unsigned long long* mask[4];
     int pos[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = sq.n0 + (f0 + min(4 * rg + i, nrows - 1)) / G;
-        mask[i] = a.mask + (size_t)n * a.W;
-        pos[i] = max(a.tok_pos[n], sq.start);
+    for (int r = 0; r < 4; ++r) {
+        const int n = s_tok[4 * rg + r];
+        mask[r] = a.mask + (size_t)n * a.W;
+        pos[r] = max(a.tok_pos[n], sq.start);
     }
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    // values: rows 8 wr .. 8 wr + 7 in pairs, columns 4 lane + 128 c .. + 3
-    const int wr = tid >> 5, lane = tid & 31;
-    pt_f2 acc[4][4 * NC];
+    // values: rows 8 vr .. 8 vr + 7 in pairs, columns col0 + 64 j .. + 3; the halves of the block have every other key each, or (values
+    // beyond 256, for the registers) half of the columns each
+    constexpr bool BY_KEYS = NC < 4;
+    constexpr int CN = BY_KEYS ? 2 * NC : NC;
+    const int half = tid >> 6, vr = (tid >> 4) & 3, col0 = 4 * (tid & 15) + (BY_KEYS ? 0 : 256 * half);
+    const bool v_idle = 8 * vr >= nrows;
+    pt_f2 acc[4][4 * CN];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < 4 * NC; ++c) acc[r][c] = 0ull;
+        for (int c = 0; c < 4 * CN; ++c) acc[r][c] = 0ull;
 
     for (int i = 0; i < npages; ++i) {
         const int jb = (pg0 + i) * LUMEN_PAGE, valid = valid_of(i);
@@ -199,57 +208,60 @@ attn_tree_kernel(const TreeArgs a) {
             ta_stage<T>(keys, ks, dp, (const T*)a.kcache + tile * a.d, a.d, a.layout, valid, a.vec & 1);
         }
         __syncthreads();
-        pt_f2 s2[4][4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s2[x][k] = 0ull;
-#pragma unroll 2
-        for (int e = 0; e < dp; e += 4) {
-            ulonglong2 x[4], y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(qs + (4 * rg + r) * ks + e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const ulonglong2*>(keys + (kg + 16 * k) * ks + e);
+        const bool all = jb + LUMEN_PAGE <= sq.start && a.window == 0;       // every row sees the whole page
+        if (!idle) {
+            pt_f2 s2[4][4];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s2[r][k] = pt_fma2(x[r].y, y[k].y, pt_fma2(x[r].x, y[k].x, s2[r][k]));
-        }
-        float s[4][4], corr[4];
-        const bool all = jb + LUMEN_PAGE <= sq.start && a.window == 0;       // every row sees the whole page
+                for (int k = 0; k < 4; ++k) s2[r][k] = 0ull;
+#pragma unroll 2
+            for (int e = 0; e < dp; e += 4) {
+                ulonglong2 x[4], y[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const unsigned long long seen = all ? ~0ull : tree_seen(jb, sq, mask[r], a.W, pos[r], a.window, a.tok_pos + sq.n0);
-            float top = -INFINITY;
+                for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(qs + (4 * rg + r) * ks + e);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float even, odd;
-                pt_unpair(s2[r][k], even, odd);
-                float x = (even + odd) * a.scale;
-                if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-                s[r][k] = (seen >> (kg + 16 * k)) & 1 ? x : -INFINITY;
-                top = fmaxf(top, s[r][k]);
+                for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const ulonglong2*>(keys + (kg + 16 * k) * ks + e);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s2[r][k] = pt_fma2(x[r].y, y[k].y, pt_fma2(x[r].x, y[k].x, s2[r][k]));
+            }
+            float s[4][4], corr[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const unsigned long long seen = all ? ~0ull : tree_seen(jb, sq, mask[r], a.W, pos[r], a.window, a.tok_pos + sq.n0);
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float even, odd;
+                    pt_unpair(s2[r][k], even, odd);
+                    float x = (even + odd) * a.scale;
+                    if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+                    s[r][k] = (seen >> (kg + 16 * k)) & 1 ? x : -INFINITY;
+                    top = fmaxf(top, s[r][k]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
+                corr[r] = m[r] == -INFINITY ? 0.0f : expf(m[r] - mn);
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s[r][k] = expf(s[r][k] - base);      // 0 for a masked key, also where none has been seen yet
+                    sum += s[r][k];
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                l[r] = l[r] * corr[r] + sum;
+                m[r] = mn;
             }
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
-            corr[r] = m[r] == -INFINITY ? 0.0f : expf(m[r] - mn);
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                s[r][k] = expf(s[r][k] - base);      // 0 for a masked key, also where none has been seen yet
-                sum += s[r][k];
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[r] = l[r] * corr[r] + sum;
-            m[r] = mn;
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<float4*>(ps + (kg + 16 * k) * TA_PROW + 4 * rg) = make_float4(s[0][k], s[1][k], s[2][k], s[3][k]);
+            if (kg == 0) *reinterpret_cast<float4*>(s_corr + 4 * rg) = make_float4(corr[0], corr[1], corr[2], corr[3]);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(ps + (kg + 16 * k) * TA_PROW + 4 * rg) = make_float4(s[0][k], s[1][k], s[2][k], s[3][k]);
-        if (kg == 0) *reinterpret_cast<float4*>(s_corr + 4 * rg) = make_float4(corr[0], corr[1], corr[2], corr[3]);
         __syncthreads();                          // the keys have been read, the weights are there
         if (ASYNC) {
             if (i + 1 < npages) ta_stage_async(keys, ks, (const float*)a.kcache + tile_of(i + 1) * a.d, a.d, valid_of(i + 1));
@@ -263,45 +275,47 @@ attn_tree_kernel(const TreeArgs a) {
         if (!all) {
             // a value that is no number, on a page that some row does not see whole
             bool bad = false;
-            for (int r = wr; r < valid; r += TA_THREADS / 32)
+            for (int r = warp; r < valid; r += TA_THREADS / 32)
                 for (int e = lane; e < a.dv; e += 32) bad |= !(fabsf(vals[r * VS + e]) <= 3.402823466e38f);
             any_bad = __syncthreads_or(bad);
         }
-        {
-            const ulonglong2 c01 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * wr), c23 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * wr + 4);
-            const pt_f2 c[4] = {c01.x, c01.y, c23.x, c23.y};
+        if (!v_idle) {
+            {
+                const ulonglong2 c01 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * vr), c23 = *reinterpret_cast<const ulonglong2*>(s_corr + 8 * vr + 4);
+                const pt_f2 c[4] = {c01.x, c01.y, c23.x, c23.y};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int x = 0; x < 4 * NC; ++x) acc[r][x] = pt_fma2(acc[r][x], c[r], 0ull);
-        }
+                    for (int x = 0; x < 4 * CN; ++x) acc[r][x] = pt_fma2(acc[r][x], c[r], 0ull);
+            }
 #pragma unroll 2
-        for (int k = 0; k < valid; ++k) {
-            const ulonglong2 w01 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * wr);
-            const ulonglong2 w23 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * wr + 4);
-            const pt_f2 w[4] = {w01.x, w01.y, w23.x, w23.y};
+            for (int k = BY_KEYS ? half : 0; k < valid; k += BY_KEYS ? 2 : 1) {
+                const ulonglong2 w01 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * vr);
+                const ulonglong2 w23 = *reinterpret_cast<const ulonglong2*>(ps + k * TA_PROW + 8 * vr + 4);
+                const pt_f2 w[4] = {w01.x, w01.y, w23.x, w23.y};
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float4 v = *reinterpret_cast<const float4*>(vals + k * VS + 128 * c + 4 * lane);
-                const pt_f2 vv[4] = {pt_pair(v.x, v.x), pt_pair(v.y, v.y), pt_pair(v.z, v.z), pt_pair(v.w, v.w)};
-                if (any_bad) {                    // nothing of a masked value, not even 0 times infinity
+                for (int c = 0; c < CN; ++c) {
+                    const float4 v = *reinterpret_cast<const float4*>(vals + k * VS + 64 * c + col0);
+                    const pt_f2 vv[4] = {pt_pair(v.x, v.x), pt_pair(v.y, v.y), pt_pair(v.z, v.z), pt_pair(v.w, v.w)};
+                    if (any_bad) {                // nothing of a masked value, not even 0 times infinity
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float w0, w1;
-                        pt_unpair(w[r], w0, w1);
+                        for (int r = 0; r < 4; ++r) {
+                            float w0, w1;
+                            pt_unpair(w[r], w0, w1);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            float a0, a1, p0, p1;
-                            pt_unpair(acc[r][4 * c + x], a0, a1);
-                            pt_unpair(pt_fma2(w[r], vv[x], acc[r][4 * c + x]), p0, p1);
-                            acc[r][4 * c + x] = pt_pair(w0 != 0.0f ? p0 : a0, w1 != 0.0f ? p1 : a1);
+                            for (int x = 0; x < 4; ++x) {
+                                float a0, a1, p0, p1;
+                                pt_unpair(acc[r][4 * c + x], a0, a1);
+                                pt_unpair(pt_fma2(w[r], vv[x], acc[r][4 * c + x]), p0, p1);
+                                acc[r][4 * c + x] = pt_pair(w0 != 0.0f ? p0 : a0, w1 != 0.0f ? p1 : a1);
+                            }
                         }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[r][4 * c + x] = pt_fma2(w[r], vv[x], acc[r][4 * c + x]);
                     }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[r][4 * c + x] = pt_fma2(w[r], vv[x], acc[r][4 * c + x]);
                 }
             }
         }
@@ -311,46 +325,57 @@ attn_tree_kernel(const TreeArgs a) {
             else asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
-    const bool whole = plan.nseg == 1;
-    const long long pair0 = tree_part_base(b, sq.n0, a.width, G);
-    if (kg == 0) {
+    if (kg == 0)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 4 * rg + i, f = f0 + r;
-            if (r >= nrows) continue;
-            const int head = kvh * G + f % G;
-            if (whole) s_inv[r] = ta_close(m[i], l[i], a.sink, head);
-            else a.part_ml[(pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head] = make_float2(m[i], l[i]);
-        }
+        for (int r = 0; r < 4; ++r) s_ml[4 * rg + r] = make_float2(m[r], l[r]);
+    // the two halves' sums come together in the values' place, the even keys' first
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float* sums = vals;                           // [32][VS]
+    if (BY_KEYS && half == 1 && !v_idle) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int c = 0; c < CN; ++c) {
+                float x[4][2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pt_unpair(acc[r >> 1][4 * c + i], x[i][0], x[i][1]);
+                *reinterpret_cast<float4*>(sums + (8 * vr + r) * VS + 64 * c + col0) = make_float4(x[0][r & 1], x[1][r & 1], x[2][r & 1], x[3][r & 1]);
+            }
     }
     __syncthreads();
+    if ((BY_KEYS && half == 1) || v_idle) return;
+    const bool whole = plan.nseg == 1;
+    const long long pair0 = tree_part_base(b, sq.n0, a.width, G);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        const int row = 8 * wr + r, f = f0 + row;
-        if (row >= nrows) continue;
-        const int head = kvh * G + f % G;
-        const float inv = whole ? s_inv[row] : 1.0f;
-        T* dst = (T*)a.out + ((size_t)(sq.n0 + f / G) * a.nq + head) * a.dv;
-        float* part = a.part_o + ((pair0 + (long long)(f / G) * plan.nseg + seg) * a.nq + head) * (long long)a.dv;
+        const int row = 8 * vr + r;
+        if (row >= nrows) break;
+        const int tok = s_tok[row], head = s_head[row];
+        const float2 ml = s_ml[row];
+        const long long at = (pair0 + (long long)(tok - sq.n0) * plan.nseg + seg) * a.nq + head;
+        const float inv = whole ? ta_close(ml.x, ml.y, a.sink, head) : 1.0f;
+        if (!whole && col0 == 0) a.part_ml[at] = ml;
+        T* dst = (T*)a.out + ((size_t)tok * a.nq + head) * a.dv;
+        float* part = a.part_o + at * a.dv;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int e = 4 * lane + 128 * c;
-            float v[4];
+        for (int c = 0; c < CN; ++c) {
+            const int e = 64 * c + col0;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (BY_KEYS) y = *reinterpret_cast<const float4*>(sums + row * VS + e);
+            float x[4][2];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                float even, odd;
-                pt_unpair(acc[r >> 1][4 * c + x], even, odd);
-                v[x] = (r & 1 ? odd : even) * inv;
-            }
+            for (int i = 0; i < 4; ++i) pt_unpair(acc[r >> 1][4 * c + i], x[i][0], x[i][1]);
+            const float v[4] = {x[0][r & 1] + y.x, x[1][r & 1] + y.y, x[2][r & 1] + y.z, x[3][r & 1] + y.w};
             if (!whole && (a.dv & 3) == 0) {
                 if (e < a.dv) *reinterpret_cast<float4*>(part + e) = make_float4(v[0], v[1], v[2], v[3]);
                 continue;
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (e + x < a.dv) {
-                    if (whole) dst[e + x] = from_f32<T>(v[x]);
-                    else part[e + x] = v[x];
+            for (int i = 0; i < 4; ++i)
+                if (e + i < a.dv) {
+                    if (whole) dst[e + i] = from_f32<T>(v[i] * inv);
+                    else part[e + i] = v[i];
                 }
         }
     }

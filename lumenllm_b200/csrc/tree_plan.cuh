@@ -34,7 +34,7 @@ __device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg
 }
 // The general kernel's cut of them: nseg segments of per or per + 1 pages (the first rem have one more).
 // A segment's partial result is rows x dv float32, its keys and values are pages x 64 x (d + dv) numbers: with a page for
-// sixteen rows at least, partials come to an eighth (float32) or a quarter of what the segment reads. The cut depends on the
+// 32 rows at least, float32 partials come to a quarter of what the segment reads, beside a time that its arithmetic takes. The cut depends on the
 // sequence alone, never on its neighbours in the batch or the page table's width.
 struct TreePlan {
     int pg_lo, np, nseg, per, rem;
@@ -45,15 +45,15 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int 
     TreePlan p;
     tree_pages(s, window, p.pg_lo, p.np);
     const long long rows = (long long)s.q * G;
-    const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 15) / 16));
+    const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 31) / 32));
     p.nseg = min((p.np + seg - 1) / seg, TREE_MAX_SEGS);
     p.per = p.np / p.nseg;
     p.rem = p.np - p.per * p.nseg;
     return p;
 }
 // Partial results of sequence b lie from this (token, segment) pair on, node i's segments at i * nseg: q * nseg is at most
-// q + 16 width / G whatever the lengths are.
-__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return (16LL * width + G - 1) / G; }
+// q + 32 width / G whatever the lengths are.
+__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return (32LL * width + G - 1) / G; }
 __device__ __forceinline__ long long tree_part_base(int b, int n0, int width, int G) {
     return (long long)b * tree_part_room(width, G) + n0;
 }

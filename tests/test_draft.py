@@ -147,9 +147,9 @@ def test_segments_of_partial_results_fit_their_room():
     for _ in range(3000):
         width, G = rng.randint(1, 700), rng.choice([1, 2, 3, 4, 5, 8, 16, 40])
         q, np_ = rng.randint(1, 300), rng.randint(1, width)
-        seg = min(np_, max(2, (q * G + 15) // 16))
+        seg = min(np_, max(2, (q * G + 31) // 32))
         nseg = min(-(-np_ // seg), 64)
-        assert nseg == 1 or (width > 2 and q * nseg <= q + -(-16 * width // G))
+        assert nseg == 1 or (width > 2 and q * nseg <= q + -(-32 * width // G))
 
 
 def drafting_engine(**over):
