@@ -191,31 +191,34 @@ attn_tree_tc_kernel(const TreeTc t) {
     {
         TreeWork w = tt_work_of(a, threadIdx.x * run, G);
         const TreeWork w0 = w;
-        int mine = w.all;
-        for (int i = 1; i < run; ++i) mine += tt_work_of(a, threadIdx.x * run + i, G).all;
-        int sum = mine;
+        long long all = w.all;
+        for (int i = 1; i < run; ++i) all += tt_work_of(a, threadIdx.x * run + i, G).all;
+        // what the host has room for fits 32 bits; lengths that come to more contradict the number of tokens, and nothing is done
+        const int mine = all < (1 << 30) ? (int)all : 1 << 30;
+        unsigned sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum = min(sum + v, 1u << 30);
         }
-        if (lane == 31) s_sum[warp] = sum;
+        if (lane == 31) s_sum[warp] = (int)sum;
         __syncthreads();
-        int total = 0;
-        sum -= mine;
+        unsigned total = 0;
 #pragma unroll
-        for (int i = 0; i < TT_THREADS / 32; ++i) {
-            if (i == warp) sum += total;
-            total += s_sum[i];
-        }
-        const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, TT_SHARE);
+        for (int i = 0; i < TT_THREADS / 32; ++i) total = min(total + (unsigned)s_sum[i], 1u << 30);
+        if (total >= 1u << 30) total = 0;
+        int before = (int)sum - mine;                   // the work ahead of this thread's
+#pragma unroll
+        for (int i = 0; i < TT_THREADS / 32; ++i)
+            if (i < warp) before += s_sum[i];
+        const int share = max((int)((total + gridDim.x - 1) / gridDim.x), TT_SHARE);
 #pragma unroll 1
         for (int end = 0; end < 2; ++end) {
             int x = ((int)blockIdx.x + end) * share;
             TreeCut cut = {a.B, 0, 0};
-            if (x >= total ? threadIdx.x != 0 : x < sum || x >= sum + mine) continue;
-            if (x < total) {
-                x -= sum;
+            if (x >= (int)total ? threadIdx.x != 0 : x < before || x >= before + mine) continue;
+            if (x < (int)total) {
+                x -= before;
                 cut.b = threadIdx.x * run;
                 w = w0;
                 while (x >= w.all) {
@@ -768,7 +771,7 @@ static cudaError_t tt_go(const TreeTc& t, int blocks, cudaStream_t stream) {
 
 // Whether the kernel takes these arguments (beside the operands' places, which bulk copies and its wide stores need).
 static bool tt_takes(int is_bf16, int B, int N, int width, int nq, int nkv, int d, int dv, int layout, int v_layout, float scale) {
-    // the work and a sequence's rows are counted in 32 bits
+    // the work and a sequence's rows are counted in 30 bits
     const long long work = ((long long)N * (nq / nkv) / PT_ROWS + B) * nkv * ((long long)width + TT_COST);
     return work < (1 << 30) && (long long)N * (nq / nkv) < (1 << 30) && is_bf16 && layout == LUMEN_LAYOUT_SW128 && v_layout == LUMEN_LAYOUT_SW128 && d <= 256 && dv <= 256 && scale > 0.0f;
 }

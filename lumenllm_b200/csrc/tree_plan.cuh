@@ -96,7 +96,7 @@ __device__ __forceinline__ unsigned long long tree_seen(int jb, const TreeSeq& s
     const int cached = s.start - jb;                      // keys of this page before the nodes
     if (cached > 0) {
         bits = cached >= 64 ? ~0ull : (1ull << cached) - 1;
-        const int lo = window > 0 ? p - window + 1 - jb : 0;        // keys before it are out of the window
+        const long long lo = window > 0 ? (long long)p - window + 1 - jb : 0;        // keys before it are out of the window
         if (lo >= 64) bits = 0;
         else if (lo > 0) bits &= ~0ull << lo;
     }

@@ -2074,6 +2074,7 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
         raise KernelError(f"attn_tree: window {window}, softcap {softcap}, {B} sequences")
     _page_table("attn_tree", block_table, B)
     words = tree_mask.shape[1]
+    window = int(window) if window < 1 << 31 else 0          # wider than any two positions are apart: every key
     _arrays("attn_tree", ("q", q, dtype, 0), ("kcache", kcache, dtype, 0), ("vcache", vcache, dtype, 0), ("cu_q", cu_q, I32, 1),
             ("seq_start", seq_start, I32, B), ("tok_seq", tok_seq, I32, N), ("tok_pos", tok_pos, I32, N),
             ("tree_mask", tree_mask, I64, N * words))
@@ -2096,7 +2097,7 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
     scratch = q.new_empty((scratch_k * 1024,), dtype=F32) if scratch_k > 0 else None
     f = fn("attn_tree", "lumen_attn_tree", _ATTN_TREE_ARGS)
     check(f(pq, pk, pv, ptr(block_table), block_table.stride(0), width, ptr(cu_q), ptr(seq_start), ptr(tok_seq), ptr(tok_pos),
-            ptr(tree_mask), words, po, tc, ptr(scratch), scratch_k, bf16, B, N, n_pages, nq, nkv, d, dv, int(window), float(scale),
+            ptr(tree_mask), words, po, tc, ptr(scratch), scratch_k, bf16, B, N, n_pages, nq, nkv, d, dv, window, float(scale),
             float(softcap), ptr(sink), int(layout), int(v_layout), ptr(error_flag(q.device)), stream_ptr()), "attn_tree")
     return out
 

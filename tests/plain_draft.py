@@ -179,7 +179,7 @@ class Case:
         of their sizes at most (2^-23: sums that drop bits), its cap by softcap 2^-20; a weight by twice that beside the
         normalising sum's own error, and by 2^-21 for its exponential; n weights and products are added in float32. Results are
         rounded to the type, half a step; the tensor cores take weights of half a step of bfloat16 too."""
-        scale = self.d ** -0.5 if scale is None else scale
+        scale = self.d ** -0.5 if scale is None else abs(scale)          # a score is off by its size, whatever its sign
         n = max(s + q for s, q in zip(self.starts, self.qlens))
         qk = float(self.q.float().abs().max()) * max(float(k.float().abs().max()) for k in self.k if k.numel()) * self.d
         qk = min(qk, float(self.q.double().norm(dim=-1).max()) * max(float(k.double().norm(dim=-1).max()) for k in self.k if k.numel()))

@@ -396,3 +396,85 @@ def test_the_operators_together_and_in_a_graph():
         for g_, w_ in zip([*outs, kc, vc], w):
             assert torch.equal(g_, w_)
     K.check_error_flags()
+
+
+def test_tree_attention_wherever_the_operands_lie():
+    """Queries and outputs that begin anywhere, page tables with longer rows, negative and zero scales, a window beyond any position."""
+    from lumenllm_b200.ops import kernels as K
+    for dtype, d in ((BF16, 128), (BF16, 64), (F32, 64), (F32, 36)):
+        c = D.Case([70, 200], [9, 33], 4, 2, d, dtype=dtype, seed=12)
+        ref, size = c.reference()
+        tol = c.bound(ref, size, rounded_weights=dtype == BF16)
+        a = {n: dev(x) for n, x in c.arrays().items()}
+        layout = 1 if dtype == BF16 else 0
+        kc, vc = (dev(D.swizzled(x) if layout else x) for x in (c.kc, c.vc))
+        wide = torch.full((2, c.width + 5), -1, dtype=I32, device="cuda")
+        wide[:, :c.width] = a["block_table"]
+        n = c.q.numel()
+        for off, out_off in ((0, 0), (8, 0), (1, 0), (0, 8), (0, 1), (3, 5)):
+            q = torch.empty((n + off,), dtype=dtype, device="cuda")[off:].view(c.q.shape).copy_(c.q)
+            out = torch.empty((n + out_off,), dtype=dtype, device="cuda")[out_off:].view(c.q.shape)
+            got = K.attn_tree(q, kc, vc, wide[:, :c.width], a["cu_q"], a["seq_start"], a["tok_seq"], a["tok_pos"], a["tree_mask"], 1 << 40,
+                              d ** -0.5, layout=layout, out=out)
+            assert got.data_ptr() == out.data_ptr() and bool(((got.cpu().double() - ref).abs() <= tol).all())
+        for scale in (-0.25, 0.0):
+            close(c, attend(c, scale=scale), scale=scale)
+        close(c, attend(c, window=(1 << 31) - 1), window=(1 << 31) - 1)
+    K.check_error_flags()
+
+
+def test_more_nodes_than_masks_cover_and_lengths_that_contradict_one_another():
+    from lumenllm_b200.ops import kernels as K
+    for dtype, d in ((BF16, 64), (F32, 64)):
+        # 300 nodes: the masks name the first 256, the others see those and are seen by nobody
+        sets = [[set(m for m in range(0, min(i, 256), 7)) | ({i} if i < 256 else set()) for i in range(300)]]
+        c = D.Case([40], [300], 2, 1, d, dtype=dtype, seed=3, words=4, sets=sets)
+        close(c, attend(c))
+        # sequences that claim the same tokens over and over: no fault, no wait that runs out
+        c = D.Case([100] * 6, [5] * 6, 2, 1, d, dtype=dtype, seed=4)
+        attend(c, cu_q=torch.tensor([0, 30, 0, 30, 0, 1 << 30, -5], dtype=I32))
+        K.check_error_flags()
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: the results are those of calls one behind the other."""
+    from lumenllm_b200.ops import kernels as K
+    cases = [D.Case([900, 50], [30, 7], 8, 2, 128, seed=s) for s in (1, 2)]
+    want = [attend(c) for c in cases]
+    held = []
+    for c in cases:
+        a = {n: dev(x) for n, x in c.arrays().items()}
+        held.append((dev(c.q), dev(D.swizzled(c.kc)), dev(D.swizzled(c.vc)), a))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            q, kc, vc, a = held[i]
+            with torch.cuda.stream(s):
+                got[i].append(K.attn_tree(q, kc, vc, a["block_table"], a["cu_q"], a["seq_start"], a["tok_seq"], a["tok_pos"],
+                                          a["tree_mask"], 0, 128 ** -0.5, layout=1))
+    torch.cuda.synchronize()
+    for i, w in enumerate(want):
+        assert all(torch.equal(x.cpu(), w) for x in got[i])
+    K.check_error_flags()
+
+
+def test_empty_steps():
+    from lumenllm_b200.ops import kernels as K
+    t = lambda *x: torch.tensor(x, dtype=I32, device="cuda")
+    none = torch.empty((0,), dtype=I32, device="cuda")
+    kc = torch.zeros((2, 1, 64, 64), dtype=BF16, device="cuda")
+    got = K.step_tables(none, none, t(1, 2).view(1, 2), none, 3, 2, parents=t(0, 0, 0))
+    assert got.cu_q.tolist() == [0] and got.tok_seq.tolist() == [0] * 3 and got.block_table.tolist() == [[0, 0]]
+    q = torch.zeros((0, 2, 64), dtype=BF16, device="cuda")
+    mask = torch.zeros((0, 1), dtype=I64, device="cuda")
+    assert K.attn_tree(q, kc, kc, t(1, 1).view(1, 2), t(0, 0), t(5), none, none, mask, 0, 1.0, layout=1).shape == (0, 2, 64)
+    out = torch.full((3, 2, 64), 2.0, dtype=BF16, device="cuda")
+    q = torch.zeros((3, 2, 64), dtype=BF16, device="cuda")
+    mask = torch.zeros((3, 1), dtype=I64, device="cuda")
+    K.attn_tree(q, kc, kc, t(1, 1).view(1, 2), t(0, 0), t(5), t(0, 0, 0), t(0, 0, 0), mask, 0, 1.0, layout=1, out=out)      # nobody's tokens
+    assert bool((out == 2.0).all())
+    count, path, said = K.tree_accept(none, none, none, t(0), 4)
+    assert count.shape == (0,) and path.shape == (0, 4) and said.shape == (0, 4)
+    K.cache_compact(kc, kc, t(1, 1).view(1, 2), t(0), path, count, layout=1)
