@@ -5,9 +5,9 @@
 // behind the cached tokens, not its index in the cache). A row that sees no key is 0. Keys and values of masked places never
 // reach a result, whatever they hold.
 //
-// This file: the general kernel (float32 and bfloat16, any key and value size up to 512, any head ratio, both tile
-// layouts; all arithmetic float32 with expf and tanhf), and the kernel that joins the segments of both this one and
-// the tensor-core kernel of attn_tree_tc.cu.
+// Three kernels. Swizzled bfloat16 pages go to the 5th-generation tensor cores (attn_tree_tc.cuh), bfloat16 pages in plain rows to
+// mma.sync (attn_tree_mma.cuh); this file has the general kernel (float32 and bfloat16, any key and value size up to 512, any
+// head ratio, both tile layouts; all arithmetic float32 with expf and tanhf), and what joins the segments of it and of the second.
 //
 // General kernel: a block has 32 rows (node, query head) of one kv head and a segment of the keys, and takes a page (64 keys)
 // at a time through shared memory in float32: scores by register tiles of 4 rows x 4 keys (the two float32 products of one instruction
@@ -38,7 +38,7 @@ struct TreeArgs {
     float* part_o;                // [pairs][nq][dv]
     float2* part_ml;              // [pairs][nq]: running maximum and sum
     const float* sink;
-    int bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec;
+    int bt_stride, width, W, B, N, n_pages, nq, nkv, d, dv, window, layout, v_layout, vec, seg_min, seg_rows;
     float scale, softcap;
 };
 
@@ -124,7 +124,7 @@ attn_tree_kernel(const TreeArgs a) {
     const int b = s_unit[0];
     if (b >= a.B) return;
     const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, b, a.N, a.width);
-    const TreePlan plan = tree_plan(sq, a.window, G);
+    const TreePlan plan = tree_plan(sq, a.window, G, a.seg_min, a.seg_rows);
     if (seg >= plan.nseg) return;
     const int f0 = s_unit[1] * TA_ROWS, nrows = min(TA_ROWS, sq.q * G - f0);
     const int dp = (a.d + 3) & ~3, ks = dp + 4;
@@ -397,7 +397,7 @@ attn_tree_join_kernel(const TreeArgs a, const int* __restrict__ tok_seq) {
     const int G = a.nq / a.nkv;
     const TreeSeq sq = tree_seq(a.cu_q, a.seq_start, b, a.N, a.width);
     if (n < sq.n0 || n >= sq.n0 + sq.q) return;
-    const TreePlan plan = tree_plan(sq, a.window, G);
+    const TreePlan plan = tree_plan(sq, a.window, G, a.seg_min, a.seg_rows);
     if (plan.nseg == 1) return;                   // done by its own block
     const int quads = (a.dv + 3) / 4, idx = blockIdx.y * 128 + threadIdx.x;
     if (idx >= a.nq * quads) return;
@@ -475,6 +475,7 @@ static cudaError_t ta_go(const TreeArgs& a, const int* tok_seq, int max_segs, cu
     return ta_run<T, NC, false>(a, tok_seq, one, max_segs, stream);
 }
 
+#include "attn_tree_mma.cuh"
 #include "attn_tree_tc.cuh"
 
 // Segments that a page table of `width` pages may be cut into.
@@ -521,13 +522,15 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
                     (((uintptr_t)q & 15) == 0 && d * es % 16 == 0 ? 4 : 0);
     // the maxima and sums first: the rows behind them lie on 16 bytes where dv is a multiple of 4
     const long long pairs = ((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2;
-    const TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out,
+    TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out,
                         scratch ? scratch + pairs * nq * 2 : nullptr, (float2*)scratch, sink, bt_stride, width, W, B, N, n_pages, nq, nkv,
-                        d, dv, window, layout, v_layout, vec, scale, softcap};
+                        d, dv, window, layout, v_layout, vec, TREE_MIN_SEG, TREE_SEG_ROWS, scale, softcap};
+    const bool mma = !tc && tm_takes(a, is_bf16);
+    if (mma) { a.seg_min = 4; a.seg_rows = 16; }
     cudaError_t e;
 #define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, tok_seq, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, tok_seq, max_segs, stream) \
                                                                                    : ta_go<T, 4>(a, tok_seq, max_segs, stream))
-    e = tc ? tt_launch(a, scratch, err, stream) : is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
+    e = tc ? tt_launch(a, scratch, err, stream) : mma ? tm_go(a, tok_seq, max_segs, stream) : is_bf16 ? TA_GO(__nv_bfloat16) : TA_GO(float);
 #undef TA_GO
     if (e != cudaSuccess) return (int)e;
     LUMEN_LAUNCH_CHECK();

@@ -45,7 +45,7 @@ MODULES = {
     "attn_decode": (["attn_decode.cu"], ["common.cuh", "mma_utils.cuh", "qk_head.cuh", "attn_decode_noalloc.h"]),
     "attn_prefill": (["attn_prefill.cu"], ["common.cuh", "mma_utils.cuh"]),
     "attn_prefill_tc": (["attn_prefill_tc.cu"], ["common.cuh", "mma_utils.cuh", "tmem_attn.cuh"]),
-    "attn_tree": (["attn_tree.cu"], ["common.cuh", "mma_utils.cuh", "tmem_attn.cuh", "tree_plan.cuh", "attn_tree_tc.cuh"]),
+    "attn_tree": (["attn_tree.cu"], ["common.cuh", "mma_utils.cuh", "tmem_attn.cuh", "tree_plan.cuh", "attn_tree_mma.cuh", "attn_tree_tc.cuh"]),
     "draft": (["draft.cu"], ["common.cuh", "tree_plan.cuh"]),
     "stream_probe": (["stream_probe.cu"], ["common.cuh", "mma_utils.cuh"]),     # a measurement (kbench stream)
 }

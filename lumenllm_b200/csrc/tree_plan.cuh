@@ -9,6 +9,7 @@
 #define TREE_MAX_NODES 256        // nodes of a sequence that the masks and the walk cover
 #define TREE_MAX_SEGS 64          // a sequence is never cut into more segments than this
 #define TREE_MIN_SEG 2            // pages of the shortest segment
+#define TREE_SEG_ROWS 32          // rows that have a page of a segment to themselves, at most
 
 struct TreeSeq {
     int n0, q;        // its first token of the step, its nodes
@@ -32,28 +33,29 @@ __device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg
     pg_lo = lo / LUMEN_PAGE;
     np = max((s.end - 1) / LUMEN_PAGE - pg_lo + 1, 1);
 }
-// The general kernel's cut of them: nseg segments of per or per + 1 pages (the first rem have one more).
-// A segment's partial result is rows x dv float32, its keys and values are pages x 64 x (d + dv) numbers: with a page for
-// 32 rows at least, float32 partials come to a quarter of what the segment reads, beside a time that its arithmetic takes. The cut depends on the
-// sequence alone, never on its neighbours in the batch or the page table's width.
+// The cut of them that does not depend on the step: nseg segments of per or per + 1 pages (the first rem have one more), of
+// seg_min pages at least and one for every seg_rows rows. A segment's partial result is rows x dv float32, its keys and values
+// are pages x 64 x (d + dv) numbers: with a page for 32 rows float32 partials come to a quarter of what the segment reads, beside a time
+// that its arithmetic takes; with one for 16 rows bfloat16 ones to as much. Never on the neighbours in the batch or the page table's
+// width.
 struct TreePlan {
     int pg_lo, np, nseg, per, rem;
     __device__ __forceinline__ int first(int seg) const { return pg_lo + seg * per + min(seg, rem); }
     __device__ __forceinline__ int count(int seg) const { return per + (seg < rem ? 1 : 0); }
 };
-__device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int G) {
+__device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int G, int seg_min, int seg_rows) {
     TreePlan p;
     tree_pages(s, window, p.pg_lo, p.np);
     const long long rows = (long long)s.q * G;
-    const int seg = (int)min((long long)p.np, max((long long)TREE_MIN_SEG, (rows + 31) / 32));
+    const int seg = (int)min((long long)p.np, max((long long)seg_min, (rows + seg_rows - 1) / seg_rows));
     p.nseg = min((p.np + seg - 1) / seg, TREE_MAX_SEGS);
     p.per = p.np / p.nseg;
     p.rem = p.np - p.per * p.nseg;
     return p;
 }
 // Partial results of sequence b lie from this (token, segment) pair on, node i's segments at i * nseg: q * nseg is at most
-// q + 32 width / G whatever the lengths are.
-__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return (32LL * width + G - 1) / G; }
+// q + TREE_SEG_ROWS width / G whatever the lengths are (seg_min TREE_MIN_SEG or more, seg_rows TREE_SEG_ROWS or less).
+__host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return ((long long)TREE_SEG_ROWS * width + G - 1) / G; }
 __device__ __forceinline__ long long tree_part_base(int b, int n0, int width, int G) {
     return (long long)b * tree_part_room(width, G) + n0;
 }
