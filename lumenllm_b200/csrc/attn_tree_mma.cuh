@@ -27,7 +27,7 @@ __device__ __forceinline__ void tm_stage(unsigned char* dst, int stride, const _
 
 // VT: values of up to 8 VT columns.
 template <int VT>
-__global__ void __launch_bounds__(TM_THREADS, VT == 16 ? 3 : 1)
+__global__ void __launch_bounds__(TM_THREADS, VT == 16 ? 3 : 0)
 attn_tree_mma_kernel(const TreeArgs a) {
     pdl_wait();      // nothing of this kernel touches global memory before this
     pdl_trigger();
