@@ -39,7 +39,8 @@ class StepEntry:
 class DraftEntry:
     """One sequence of a step that checks drafts: its slot, the tokens of a tree and the parent of each, a number of an
     earlier one. tokens[0] is certain (the token that was sampled last and is not in the cache yet; parents[0] is
-    -1); the others are drafted: a path from the first down is a continuation that may be accepted."""
+    -1); the others are drafted: a path from the first down is a continuation that may be accepted. A token's position is the
+    sequence's cached length plus its depth in the tree."""
     slot: int
     tokens: Sequence[int]
     parents: Sequence[int]

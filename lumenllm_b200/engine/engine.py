@@ -253,7 +253,7 @@ class Engine:
         the one picked behind the last of them, so one at least. The cache then holds the first token and the kept
         ones; the last returned token is not in it: it is the next step's first.
         `configs`: a SamplingConfig a sequence (without: greedy). `uniforms`: for each sequence as many numbers in [0, 1)
-        as its tree is deep, number k for the token picked at depth k: with the numbers that single steps would have drawn,
+        as its tree is deep, number k for the token picked at depth k (a greedy sequence's row is not read and may be None): with the numbers that single steps would have drawn,
         the tokens are those of single steps (up to the rounding of logits)."""
         drafts = [e if isinstance(e, DraftEntry) else DraftEntry(*e) for e in drafts]
         depths = self._validate_drafts(drafts, configs, uniforms)
@@ -267,8 +267,8 @@ class Engine:
             picked = K.argmax(logits)
         else:
             picked = self.sampler.pick(logits, [c for c, d in zip(configs, depths) for _ in d],
-                                       [0.0 if u is None else float(u[x]) for u, d in
-                                        zip(uniforms or [None] * len(drafts), depths) for x in d])
+                                       [0.0 if c.greedy else float(u[x]) for c, u, d in
+                                        zip(configs, uniforms or [None] * len(drafts), depths) for x in d])
         count, path, emitted = K.tree_accept(picked, ctx.tokens, parents, ctx.cu_q, 1 + max(max(d) for d in depths))
         for g, table in zip(self.cache.groups, ctx.block_tables):
             K.cache_compact(g.k, None if g.need.values_in_keys else g.v, table, ctx.seq_start, path, count, layout=g.layout,
@@ -304,8 +304,10 @@ class Engine:
             d = [0]
             for p in e.parents[1:]:
                 d.append(d[int(p)] + 1)
-            if configs is not None and uniforms is not None and not configs[i].greedy and len(uniforms[i]) <= max(d):
-                raise StepError(f"slot {e.slot}: {len(uniforms[i])} uniform numbers for a tree {max(d) + 1} tokens deep")
+            if configs is not None and not configs[i].greedy:
+                given = 0 if uniforms[i] is None else len(uniforms[i])
+                if given <= max(d):
+                    raise StepError(f"slot {e.slot}: {given} uniform numbers for a tree {max(d) + 1} tokens deep")
             depths.append(d)
         return depths
 

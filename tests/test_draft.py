@@ -181,6 +181,7 @@ def drafting_engine(**over):
     ([(0, [1, 2], [-1, 0])], dict(configs=["hot"]), "uniform numbers"),
     ([(0, [1, 2], [-1, 0])], dict(configs=["hot"], uniforms=[[0.5]]), "2 tokens deep"),
     ([(0, [1, 2], [-1, 0])], dict(configs=["cold"], uniforms=[[0.5], [0.5]]), "one row of uniform numbers"),
+    ([(0, [1, 2], [-1, 0]), (1, [1], [-1])], dict(configs=["cold", "hot"], uniforms=[[0.5, 0.5], None]), "0 uniform numbers"),
 ])
 def test_verify_refuses(drafts, kw, says):
     from lumenllm_b200 import DraftEntry, SamplingConfig, StepError

@@ -117,6 +117,20 @@ def test_sampled_drafts_are_sampled_steps(engines):
         eng.free_slot(slots[b])
 
 
+def test_a_greedy_sequence_among_sampled_ones_needs_no_numbers(engines):
+    from lumenllm_b200 import DraftEntry, SamplingConfig, StepEntry
+    eng = engines("A", "float32")
+    prompts = seeded_tokens(TINY["A"]["vocab_size"], [20, 31], seed=9)
+    alone, cfgs = [], [SamplingConfig(), SamplingConfig(temperature=0.9, seed=2)]
+    for rows in ([[0.1, 0.2], [0.3, 0.4]], [None, [0.3, 0.4]], [[], [0.3, 0.4]]):
+        slots = [eng.alloc_slot() for _ in prompts]
+        eng.step([StepEntry(s, p[:-1], []) for s, p in zip(slots, prompts)])
+        alone.append(eng.verify([DraftEntry(s, [p[-1], 5], [-1, 0]) for s, p in zip(slots, prompts)], cfgs, rows))
+        for s in slots:
+            eng.free_slot(s)
+    assert alone[0] == alone[1] == alone[2]
+
+
 def test_drafts_between_ordinary_steps_and_a_full_cache(tiny_models):
     """verify, step and generate share the slots; a step of drafts for which there is no room is refused and changes nothing."""
     from lumenllm_b200 import DraftEntry, Engine, GenerateRequest, StepEntry, StepError
