@@ -3,6 +3,7 @@
     python -m lumenllm_b200.kbench gemm_tc --m 2048 --n 4096 --k 4096 [--silu] [--copies 8] [--reps 5]
     python -m lumenllm_b200.kbench attn_decode --batch 8 --len 1600 --heads 32 --kv-heads 8 --head-dim 128
     python -m lumenllm_b200.kbench attn_prefill --tokens 2048 --heads 32 --kv-heads 8 --head-dim 128
+    python -m lumenllm_b200.kbench attn_tree --batch 8 --len 2000 --nodes 64 --heads 32 --kv-heads 8 --head-dim 128
     python -m lumenllm_b200.kbench add_rmsnorm --m 2048 --n 4096 [--splits 9]
     python -m lumenllm_b200.kbench qk_rope --m 2048 --heads 32 --kv-heads 8 --head-dim 128
     python -m lumenllm_b200.kbench gemm_qkv --m 2048 --k 4096 --heads 32 --kv-heads 8
@@ -60,7 +61,7 @@ def _paged(B, length, nkv, d, dev):
 
 def main(argv=None):
     ap = argparse.ArgumentParser(prog="kbench")
-    ap.add_argument("kernel", choices=["gemm_tc", "attn_decode", "attn_prefill",
+    ap.add_argument("kernel", choices=["gemm_tc", "attn_decode", "attn_prefill", "attn_tree",
                                        "add_rmsnorm", "qk_rope", "gemm_qkv", "argmax", "sample", "stream"])
     ap.add_argument("--splits", type=int, default=1, help="add_rmsnorm: partial sums to add")
     ap.add_argument("--top-k", type=int, default=0)
@@ -73,6 +74,7 @@ def main(argv=None):
     ap.add_argument("--mma-sync", action="store_true", help="attn_prefill: the mma.sync kernel")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--len", type=int, default=1600)
+    ap.add_argument("--nodes", type=int, default=64, help="attn_tree: nodes of each sequence's tree, --len tokens before it")
     ap.add_argument("--tokens", type=int, default=2048)
     ap.add_argument("--heads", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=8)
@@ -151,6 +153,24 @@ def main(argv=None):
         us = _time(fns, a.reps)
         flops = 2.0 * a.tokens * a.tokens * a.head_dim * a.heads      # causal: half of 4 T^2 d
         note = f"{flops / us / 1e6:.1f} TFLOP/s"
+    elif a.kernel == "attn_tree":
+        sets = [_paged(a.batch, a.len + a.nodes, a.kv_heads, a.head_dim, dev) for _ in range(a.copies)]
+        q = torch.randn(a.batch * a.nodes, a.heads, a.head_dim, device=dev).to(bf)
+        parents = [(i - 1) // 2 for i in range(a.nodes)] * a.batch          # two children a node
+        depth = [0] * a.nodes
+        for i in range(1, a.nodes):
+            depth[i] = depth[parents[i]] + 1
+        st = torch.full((a.batch,), a.len, dtype=torch.int32, device=dev)
+        t = K.step_tables(st, torch.full_like(st, a.nodes), sets[0][2], torch.arange(a.batch, dtype=torch.int32, device=dev),
+                          a.batch * a.nodes, sets[0][2].shape[1], torch.tensor(parents, dtype=torch.int32, device=dev),
+                          (a.nodes + 63) // 64)
+        fns = [lambda s=s: K.attn_tree(q, s[0], s[1], t.block_table, t.cu_q, st, t.tok_seq, t.tok_pos, t.tree_mask, 0,
+                                       a.head_dim ** -0.5, layout=K.LAYOUT_SW128 if a.head_dim % 64 == 0 else K.LAYOUT_LINEAR)
+               for s in sets]
+        us = _time(fns, a.reps)
+        nbytes = a.batch * (2 * (a.len + a.nodes) * a.kv_heads + 2 * a.nodes * a.heads) * a.head_dim * 2
+        flops = 4.0 * a.batch * (a.nodes * a.len + sum(depth) + a.nodes) * a.head_dim * a.heads
+        note = f"{nbytes / us / 1e3:.0f} GB/s  {flops / us / 1e6:.1f} TFLOP/s"
     elif a.kernel == "add_rmsnorm":
         hs = [torch.randn(a.m, a.n, device=dev) for _ in range(a.copies)]
         ds = [torch.randn(a.splits, a.m, a.n, device=dev) for _ in range(a.copies)]

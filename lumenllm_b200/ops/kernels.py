@@ -2050,7 +2050,8 @@ def attn_tree(q, kcache, vcache, block_table, cu_q, seq_start, tok_seq, tok_pos,
     position is its index). Scores are scale * q . k, with softcap c > 0 then c tanh(score / c); `sink` (float32 [nq], or True for
     zeros) adds exp(sink[head]) to the softmax's denominator. A row that sees nothing is 0. What a masked key or value holds does
     not matter, infinities and NaN included. Rows behind the last sequence (cu_q[B]) are not written; `out` takes the result.
-    Keys and values up to 512 numbers, any nq that is a multiple of nkv."""
+    Keys and values up to 512 numbers, any nq that is a multiple of nkv. The same step gives the same bits; on swizzled tiles,
+    whose kernel deals the work of all sequences out evenly, a sequence's last bits also depend on the others of its step."""
     N, nq, d = q.shape
     dtype = q.dtype
     if (dtype is not BF16 and dtype is not F32) or kcache.dtype is not dtype or vcache.dtype is not dtype:

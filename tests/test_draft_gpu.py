@@ -478,3 +478,12 @@ def test_empty_steps():
     count, path, said = K.tree_accept(none, none, none, t(0), 4)
     assert count.shape == (0,) and path.shape == (0, 4) and said.shape == (0, 4)
     K.cache_compact(kc, kc, t(1, 1).view(1, 2), t(0), path, count, layout=1)
+
+
+@pytest.mark.parametrize("args", [["--batch", "2", "--len", "200"], ["--batch", "1", "--len", "70", "--nodes", "130"],
+                                  ["--batch", "2", "--len", "100", "--nodes", "5", "--head-dim", "80"]])
+def test_the_micro_benchmark_runs_tree_attention(args, capsys):
+    from lumenllm_b200 import kbench
+    kbench.main(["attn_tree", *args, "--copies", "2", "--reps", "1"])
+    line = capsys.readouterr().out.strip().splitlines()[-1]
+    assert line.startswith("attn_tree:") and "us per launch" in line
