@@ -512,7 +512,7 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     if ((layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || d % 64)) || (v_layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || dv % 64)))
         return LUMEN_ERR_UNSUPPORTED;
     const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = ta_segs(width);
-    if (((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
+    if ((long long)N * G > (1 << 30) || ((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
     const int need = lumen_attn_tree_scratch(tc, B, N, width, nq, nkv, d, dv);
     if (need < 0) return LUMEN_ERR_UNSUPPORTED;
     if ((tc && (!tt_takes(is_bf16, B, N, width, nq, nkv, d, dv, layout, v_layout, scale) || !tt_aligned(q, kcache, vcache, out))) || scratch_k < need ||

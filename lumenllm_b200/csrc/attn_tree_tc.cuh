@@ -453,7 +453,17 @@ attn_tree_tc_kernel(const TreeTc t) {
             }
             if (ok && lane == 0) pt_mbar_arrive(&u_empty[slot]);
         }
-        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(t.err, 1); }
+        if (!ok) {
+            // its copies and products in flight end before the tensor memory is given back
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (lane == 0) {
+                *abort_flag = 1;
+                atomicExch(t.err, 1);
+                if (cs > 0) mbar_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1);
+                if (cv > 0) mbar_wait(&pv_done[(cv - 1) & 1], ((cv - 1) >> 1) & 1);
+            }
+            __syncwarp();
+        }
     } else {
         const int r = (warp & 3) * 32 + lane;            // this thread's row of a unit
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
@@ -497,25 +507,39 @@ attn_tree_tc_kernel(const TreeTc t) {
                 pt_fence_after();
                 float s[64];
                 pt_ld64(lane_addr + (c & 1) * LUMEN_PAGE, s);
+                const int jb = (pg0 + it) * LUMEN_PAGE;
+                const bool part = masked(jb);
+                uint32_t s0 = ~0u, s1 = ~0u;             // the keys that this row sees
+                if (part) {
+                    const unsigned long long seen = row_ok ? tree_seen(jb, sq, mask, a.W, prow, a.window, a.tok_pos + sq.n0) : 0ull;
+                    s0 = (uint32_t)seen;
+                    s1 = (uint32_t)(seen >> 32);
+                }
                 if (CAP) {       // capped scores: tanh here, times softcap * log2(e) (scale_log2) below
+                    if (part) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            s[j] = (s0 >> j) & 1 ? s[j] : 0.0f;
+                            s[32 + j] = (s1 >> j) & 1 ? s[32 + j] : 0.0f;
+                        }
+                    }
+                    // a row takes the one or the other by the scores of its own that it sees, whatever its neighbours have
                     float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int j = 0; j < 64; j += 8)
 #pragma unroll
                         for (int h = 0; h < 4; ++h) big[h] = pt_max3(big[h], fabsf(s[j + 2 * h]), fabsf(s[j + 2 * h + 1]));
-                    if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * t.cap_pre <= 0.5f)) {
+                    if (!row_ok || fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * t.cap_pre <= 0.5f) {
 #pragma unroll
                         for (int j = 0; j < 64; j += 2) tt_tanh_small(s[j], s[j + 1], t.cap_pre);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) s[j] = pt_tanh(s[j] * t.cap_pre);
                     }
+                    __syncwarp();
                 }
-                const int jb = (pg0 + it) * LUMEN_PAGE;
-                if (masked(jb)) {
+                if (part) {
                     any_masked = true;
-                    const unsigned long long seen = row_ok ? tree_seen(jb, sq, mask, a.W, prow, a.window, a.tok_pos + sq.n0) : 0ull;
-                    const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         s[j] = (s0 >> j) & 1 ? s[j] : -INFINITY;

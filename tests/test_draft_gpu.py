@@ -125,6 +125,31 @@ def test_masked_numbers_never_reach_a_result(dtype, d, what):
             n += 1
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 128), (BF16, 80), (F32, 64)])
+@pytest.mark.parametrize("window", [0, 150])
+def test_masked_numbers_do_not_move_a_bit(dtype, d, window):
+    """Large numbers in places that a row does not see, and whatever calls before left in shared memory, under a cap on the scores."""
+    case = lambda **kw: D.Case([200, 5], [30, 6], 4, 2, d, dtype=dtype, seed=9, **kw)
+    c = case()
+    want = attend(c, window, 20.0)
+    hurt = {(0, 203), (0, 10), (1, 5)}
+    for b, j in hurt:
+        c.k[b][j], c.v[b][j] = 300.0, 1e4
+    c.fill()
+    attend(case(q_scale=1000.0), window, 20.0)
+    got = attend(c, window, 20.0)
+    n = 0
+    for b, count in enumerate(c.qlens):
+        for i in range(count):
+            p = c.pos[b][i]
+            sees = any(bb == b and ((j >= c.starts[b] and (j - c.starts[b]) in c.sets[b][i]) or
+                                    (j < c.starts[b] and (not window or p - j < window))) for bb, j in hurt)
+            assert sees or torch.equal(got[n], want[n]), (b, i)
+            n += 1
+    attend(case(q_scale=1000.0), window, 20.0)
+    assert torch.equal(attend(case(), window, 20.0), want)
+
+
 def test_values_alone_that_are_no_numbers():
     """Finite keys with infinite values: a row that sees the key is infinite there and right elsewhere."""
     for dtype, d in ((BF16, 64), (BF16, 128), (F32, 64)):
