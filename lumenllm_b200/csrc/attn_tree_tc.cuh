@@ -15,6 +15,12 @@
 // products, warps 2 to 5 are the softmax. Pages that hold
 // nodes, or that a window cuts for some row, are masked: a row has one 64-bit word a page with the keys it sees.
 //
+// What bounds long steps is shared memory's 128 bytes a cycle: with 128 numbers a head a page is 32 KB written by the copies, 32 KB of Q
+// and 16 KB of K read by S, 16 KB of V by O, 750 cycles, of the 975 that a page takes an SM with two blocks on it (64 nodes for 8
+// sequences, 65 us). Hence P in tensor memory and not beside it: S of two pages in one product (Q is read half as often) with P in
+// shared memory, which tensor memory has no room for then, took 73 us, that with two threads a row (half of the keys each) 86. Steps of few
+// nodes are bound by HBM (16 nodes for 64 sequences: 5.6 TB/s, 0.86 of a copy).
+//
 // Weights are rounded to bfloat16 because the product takes both operands in one type: half a step, 2^-8 of a weight, which
 // the sum over the keys averages; the running sum takes them unrounded.
 //
