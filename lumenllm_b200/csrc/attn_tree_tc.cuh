@@ -36,8 +36,12 @@
 #define TT_STAGES 2
 #define TT_RESCALE 8.0f
 #define TT_BAR_WORDS 48           // 8-byte words of barriers, units and flags
-#define TT_COST 3                 // what a row block costs beside its pages, in pages
-#define TT_SHARE 3                // a block's least share of the work, in pages
+// What a row block costs beside its pages, in pages: Q, the first page's latency and the rows' writing (64 nodes for 8 sequences: 66 to 69 us;
+// with 1 or 6 pages 70).
+#define TT_COST 3
+// A block's least share of the work, in pages: fewer make more pieces to join, more leave SMs idle in small steps (8 nodes after 1,300
+// tokens: 13.1 us; with 2 pages 13.7, with 5 15.7).
+#define TT_SHARE 3
 
 // A place in the step's work: page `page` (counted from the first that the sequence's nodes see) of row block rb of sequence b.
 // b = B: the end.
@@ -721,7 +725,7 @@ attn_tree_tc_kernel(const TreeTc t) {
 // cuts share a row block's rows, a thread has four columns of a row at a time. What it takes is the latency of its loads, one behind
 // the other: those of TJ_BATCH pieces are under way together, and few registers let all blocks be resident at once.
 #define TJ_BATCH 4
-#define TJ_SLICES 4               // blocks a cut
+#define TJ_SLICES 4               // blocks a cut (16 nodes for 64 sequences: 78 us; with 2 blocks 84, with 8 80)
 __global__ void __launch_bounds__(256, 4)
 attn_tree_tc_join_kernel(const TreeTc t) {
     pdl_wait();
