@@ -15,11 +15,11 @@
 // products, warps 2 to 5 are the softmax. Pages that hold
 // nodes, or that a window cuts for some row, are masked: a row has one 64-bit word a page with the keys it sees.
 //
-// What bounds long steps is shared memory's 128 bytes a cycle: with 128 numbers a head a page is 32 KB written by the copies, 32 KB of Q
-// and 16 KB of K read by S, 16 KB of V by O, 750 cycles, of the 975 that a page takes an SM with two blocks on it (64 nodes for 8
-// sequences, 65 us). Hence P in tensor memory and not beside it: S of two pages in one product (Q is read half as often) with P in
-// shared memory, which tensor memory has no room for then, took 73 us, that with two threads a row (half of the keys each) 86. Steps of few
-// nodes are bound by HBM (16 nodes for 64 sequences: 5.6 TB/s, 0.86 of a copy).
+// What bounds long steps. Of several row blocks a kv head (64 nodes for 8 sequences, 63 us): the chain of S, softmax and O a page,
+// which the two blocks of an SM hide from one another in part; with all pages in L2 and the softmax left out it takes 54 us, with but one
+// step of each product besides 40. Of one row block (16 nodes for 64 sequences, 78 us): HBM, 5.4 TB/s here; 73 without softmax and
+// products, 67 with all pages in L2. S of two pages in one product with P in shared memory (tensor memory has no room for it then)
+// took 73 and 81 us, that with two threads a row, half of the keys each, 86 and 98.
 //
 // Weights are rounded to bfloat16 because the product takes both operands in one type: half a step, 2^-8 of a weight, which
 // the sum over the keys averages; the running sum takes them unrounded.
@@ -36,8 +36,8 @@
 #define TT_STAGES 2
 #define TT_RESCALE 8.0f
 #define TT_BAR_WORDS 48           // 8-byte words of barriers, units and flags
-// What a row block costs beside its pages, in pages: Q, the first page's latency and the rows' writing (64 nodes for 8 sequences: 66 to 69 us;
-// with 1 or 6 pages 70).
+// What a row block costs beside its pages, in pages: Q, the first page's latency and the rows' writing (64 nodes for 8 sequences, before the
+// teams: 66 to 69 us; with 1 or 6 pages 70).
 #define TT_COST 3
 // A block's least share of the work, in pages: fewer make more pieces to join, more leave SMs idle in small steps (8 nodes after 1,300
 // tokens: 13.1 us; with 2 pages 13.7, with 5 15.7).
@@ -49,9 +49,9 @@ struct TreeCut {
     int b, rb, page;
 };
 // A row block that is cut, as each of its cuts leaves it for the second kernel: its sequence's first token, its first row, kv head and
-// rows, the pieces it is in (0: this cut lies between row blocks) and the number of this cut among its own.
+// rows, the pieces it is in (0: this cut lies between row blocks), the number of this cut among its own and how many blocks apart they are.
 struct TreeJoin {
-    int n0, f0, kvh, nrows, pieces, order, unused[2];
+    int n0, f0, kvh, nrows, pieces, order, step, unused;
 };
 struct TreeTc {
     TreeArgs a;
@@ -166,7 +166,8 @@ attn_tree_tc_kernel(const TreeTc t) {
     volatile int* s_unit = s_bad + 2;          // [2][TT_UNIT_INTS]
     TreeCut* s_cut = reinterpret_cast<TreeCut*>(s_bad + 2 + 2 * TT_UNIT_INTS);      // [2] where this block's work begins and ends
     volatile int* s_sum = reinterpret_cast<volatile int*>(s_cut + 2);               // [warps]
-    volatile int* s_first = s_sum + TT_THREADS / 32;                                // [7] the first unit's sequence
+    volatile int* s_tiles = s_sum + TT_THREADS / 32;                                // [warps][2] least and most row blocks of a kv head
+    volatile int* s_first = s_tiles + 2 * (TT_THREADS / 32);                        // [7] the first unit's sequence
 
     const int G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -195,23 +196,36 @@ attn_tree_tc_kernel(const TreeTc t) {
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();      // nothing of this kernel touches global memory before this
     pdl_trigger();
+    // Row blocks of a kv head read the same pages. Where every sequence has as many of them, 2 to 4 neighbouring blocks are a team that
+    // walks the same pages at the same time, each for a row block of its own: the pages come from HBM once (64 nodes for 8 sequences:
+    // 171 MB of HBM reads and 63 us, without teams 255 and 66 to 69).
+    //
     // Every block adds up the step's work, a thread the work of `run` neighbouring sequences; the threads whose sequences hold the
     // ends of the block's share find the places there. A cut is not made within two pages of a row block's ends.
     const int run = (a.B + TT_THREADS - 1) / TT_THREADS;
+    int team = 1, in_team = 0;
     {
         TreeWork w = tt_work_of(a, threadIdx.x * run, G);
         const TreeWork w0 = w;
         long long all = w.all;
-        for (int i = 1; i < run; ++i) all += tt_work_of(a, threadIdx.x * run + i, G).all;
+        int least = w.tiles ? w.tiles : 1 << 30, most = w.tiles;
+        for (int i = 1; i < run; ++i) {
+            const TreeWork x = tt_work_of(a, threadIdx.x * run + i, G);
+            all += x.all;
+            if (x.tiles) least = min(least, x.tiles);
+            most = max(most, x.tiles);
+        }
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
         // what the host has room for fits 32 bits; lengths that come to more contradict the number of tokens, and nothing is done
-        const int mine = all < (1 << 30) ? (int)all : 1 << 30;
+        int mine = all < (1 << 30) ? (int)all : 1 << 30;
         unsigned sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum = min(sum + v, 1u << 30);
         }
-        if (lane == 31) s_sum[warp] = (int)sum;
+        if (lane == 31) { s_sum[warp] = (int)sum; s_tiles[2 * warp] = least; s_tiles[2 * warp + 1] = most; }
         __syncthreads();
         unsigned total = 0;
 #pragma unroll
@@ -221,18 +235,35 @@ attn_tree_tc_kernel(const TreeTc t) {
 #pragma unroll
         for (int i = 0; i < TT_THREADS / 32; ++i)
             if (i < warp) before += s_sum[i];
-        const int share = max((int)((total + gridDim.x - 1) / gridDim.x), TT_SHARE);
+#pragma unroll
+        for (int i = 0; i < TT_THREADS / 32; ++i) {
+            least = min(least, s_tiles[2 * i]);
+            most = max(most, s_tiles[2 * i + 1]);
+        }
+        // (with few blocks those that make no whole team would be missed, and the pages stay in L2 anyway)
+        if (least == most && most > 1 && gridDim.x >= 64) team = most % 4 == 0 ? 4 : most % 3 == 0 ? 3 : most % 2 == 0 ? 2 : 1;
+        int teams = gridDim.x, number = blockIdx.x;      // of a team's line of work, which has every team-th row block
+        if (team > 1) {
+            teams /= team;
+            number /= team;
+            in_team = blockIdx.x - number * team;
+            total /= team;
+            before /= team;
+            mine /= team;
+        }
+        auto line = [&](int x) { return team > 1 ? x / team : x; };
+        const int share = max((int)((total + teams - 1) / teams), TT_SHARE);
 #pragma unroll 1
         for (int end = 0; end < 2; ++end) {
-            int x = ((int)blockIdx.x + end) * share;
+            int x = number < teams ? (number + end) * share : (int)total;
             TreeCut cut = {a.B, 0, 0};
             if (x >= (int)total ? threadIdx.x != 0 : x < before || x >= before + mine) continue;
             if (x < (int)total) {
                 x -= before;
                 cut.b = threadIdx.x * run;
                 w = w0;
-                while (x >= w.all) {
-                    x -= w.all;
+                while (x >= line(w.all)) {
+                    x -= line(w.all);
                     w = tt_work_of(a, ++cut.b, G);
                 }
                 cut.rb = x / (w.np + TT_COST);
@@ -240,7 +271,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                 if (cut.page < 2) cut.page = 0;
                 else if (w.np - cut.page < 2) {
                     cut.page = 0;
-                    if (++cut.rb == w.tiles * a.nkv) {
+                    if (++cut.rb == line(w.tiles) * a.nkv) {
                         cut.rb = 0;
                         do w = tt_work_of(a, ++cut.b, G);
                         while (cut.b < a.B && w.all == 0);
@@ -249,7 +280,7 @@ attn_tree_tc_kernel(const TreeTc t) {
             }
             s_cut[end] = cut;
             if (end == 1) continue;
-            TreeJoin join = {0, 0, 0, 0, 0, 0, {0, 0}};
+            TreeJoin join = {0, 0, 0, 0, 0, 0, team, 0};
             if (cut.b < a.B) {
                 // what warp 0 needs for the block's first keys, and the second kernel to put the row block together
                 const TreeSeq s = tree_seq(a.cu_q, a.seq_start, cut.b, a.N, a.width);
@@ -258,8 +289,9 @@ attn_tree_tc_kernel(const TreeTc t) {
                 tt_prefetch(a.block_table + (size_t)cut.b * a.bt_stride + w.pg_lo + cut.page);
                 if (cut.page > 0) {
                     join.n0 = s.n0;
-                    join.kvh = cut.rb / w.tiles;
-                    join.f0 = (cut.rb - join.kvh * w.tiles) * PT_ROWS;
+                    const int tiles = line(w.tiles);
+                    join.kvh = cut.rb / tiles;
+                    join.f0 = ((cut.rb - join.kvh * tiles) * team + in_team) * PT_ROWS;
                     join.nrows = min(PT_ROWS, s.q * G - join.f0);
                     join.order = (cut.page - 2) / share;          // the cuts before it and behind it lie `share` pages apart
                     join.pieces = 2 + join.order + (w.np - 2 - cut.page) / share;
@@ -300,7 +332,8 @@ attn_tree_tc_kernel(const TreeTc t) {
                     sq_l = b0 + lane < a.B ? tree_seq(a.cu_q, a.seq_start, b0 + lane, a.N, a.width) : TreeSeq{0, 0, 0, 0};
                     w_l = tt_work(a, sq_l, G);
                 }
-                const int src = at.b - b0, np = __shfl_sync(0xffffffffu, w_l.np, src), tiles = __shfl_sync(0xffffffffu, w_l.tiles, src);
+                const int src = at.b - b0, np = __shfl_sync(0xffffffffu, w_l.np, src), all_tiles = __shfl_sync(0xffffffffu, w_l.tiles, src);
+                const int tiles = team > 1 ? all_tiles / team : all_tiles;
                 if (at.rb >= tiles * a.nkv) { ++at.b; at.rb = at.page = 0; continue; }
                 const bool ends = at.b == to.b && at.rb == to.rb;
                 const int last = ends ? to.page : np;
@@ -313,7 +346,7 @@ attn_tree_tc_kernel(const TreeTc t) {
                 x.pg0 = __shfl_sync(0xffffffffu, w_l.pg_lo, src) + at.page;
                 x.npages = last - at.page;
                 x.kvh = at.rb / tiles;
-                x.f0 = (at.rb - x.kvh * tiles) * PT_ROWS;
+                x.f0 = ((at.rb - x.kvh * tiles) * team + in_team) * PT_ROWS;
                 x.slot = at.page > 0 ? 0 : last < np ? 1 : -1;
                 ++at.rb;
                 at.page = 0;
@@ -734,7 +767,7 @@ attn_tree_tc_join_kernel(const TreeTc t) {
     const int i = blockIdx.x + 1, G = a.nq / a.nkv, quads = a.dv >> 2;
     const TreeJoin join = t.joins[i];
     if (join.pieces == 0) return;
-    const size_t first = (size_t)(2 * (i - join.order) - 1) * PT_ROWS;       // piece 0: slot 1 of the block before the first cut
+    const int cut0 = i - join.order * join.step;        // the block behind the first cut; piece 0 is in slot 1 of the one before it
     for (int idx = (join.order * TJ_SLICES + blockIdx.y) * 256 + threadIdx.x; idx < join.nrows * quads; idx += (join.pieces - 1) * TJ_SLICES * 256) {
         const int row = idx / quads, e = (idx - row * quads) * 4;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -748,7 +781,8 @@ attn_tree_tc_join_kernel(const TreeTc t) {
                 v[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (s0 + s < join.pieces) {
                     // the pieces behind: slot 0 of the block behind the first cut and of those that follow
-                    const size_t from = first + row + (s0 + s == 0 ? 0 : (size_t)(2 * (s0 + s) - 1) * PT_ROWS);
+                    const int block = cut0 + (s0 + s - 1) * join.step;
+                    const size_t from = (size_t)(2 * block + (s0 + s == 0 ? 1 : 0)) * PT_ROWS + row;
                     x[s] = a.part_ml[from];
                     v[s] = *reinterpret_cast<const float4*>(a.part_o + from * a.dv + e);
                 }

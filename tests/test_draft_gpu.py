@@ -215,6 +215,18 @@ def test_work_dealt_out_over_the_blocks():
         close(c, attend(c))
 
 
+@pytest.mark.parametrize("nodes,nq,nkv,d", [(64, 16, 4, 64), (100, 8, 2, 64), (48, 8, 1, 128), (16, 32, 2, 64), (17, 32, 1, 64), (250, 6, 2, 64),
+                                            (40, 16, 1, 256)])
+def test_row_blocks_of_a_kv_head_side_by_side(nodes, nq, nkv, d):
+    """Sequences of different lengths with as many row blocks each (2, 3, 4, 5, 6 and more, the last one not full), cut anywhere."""
+    c = D.Case([1500, 30, 777, 2100, 0], [nodes] * 4 + [nodes - 1], nq, nkv, d, dtype=BF16, seed=nodes)
+    got = attend(c)
+    close(c, got)
+    assert torch.equal(got, attend(c))
+    c = D.Case([900, 64, 1300], [nodes] * 3, nq, nkv, d, dtype=BF16, seed=nodes + 1)
+    close(c, attend(c, 300), window=300)
+
+
 def test_lengths_and_pages_that_cannot_be_are_held_inside_the_arrays():
     """Lengths below 0 or beyond the page table, pages that are not there, cu_q beyond the tokens: no fault, and the
     sequences beside them are right."""
