@@ -19,7 +19,7 @@ pages and groups are this library's own.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -128,6 +128,17 @@ class CacheGroup:
             self._changed.add(slot)
             self.n_held[slot] += want_end - have_end
             self.end_page[slot] = want_end
+
+    def shrink(self, slot: int, end: int) -> None:
+        """Gives back the slot's pages from number `end` on, the last one taken first, so that the pool hands them out
+        in the order it had. `end` does not lie before the window's run."""
+        have_end = int(self.end_page[slot])
+        if end < have_end:
+            self.pool.give_back(self.table[slot, end:have_end][::-1].tolist())
+            self.table[slot, end:have_end] = 0
+            self._changed.add(slot)
+            self.n_held[slot] -= have_end - end
+            self.end_page[slot] = end
 
     def trim(self, slot: int, length: int) -> None:
         """After a step: a group with a window or with chunks gives back the pages that no
@@ -248,12 +259,26 @@ class KVCache:
     # -------------------------------------------------- growth
     def reserve(self, slot: int, n_new: int) -> int:
         """Makes room for n_new more tokens of the slot; returns its current length.
-        On CacheFull the slot keeps what it had."""
-        self._live(slot)
-        cur = int(self.lengths[slot])
-        for g in self.groups:
-            g.reserve(slot, cur + n_new)
-        return cur
+        On CacheFull the slot keeps what it had, in every group."""
+        return self.reserve_all([(slot, n_new)])[0]
+
+    def reserve_all(self, wants: Sequence[Tuple[int, int]]) -> List[int]:
+        """Makes room for n_new more tokens of each (slot, n_new); returns the slots' current lengths. Where one does not
+        fit, no slot of them keeps a page that it had not before."""
+        starts, before = [], []
+        try:
+            for slot, n_new in wants:
+                self._live(slot)
+                cur = int(self.lengths[slot])
+                starts.append(cur)
+                for g in self.groups:
+                    before.append((g, slot, int(g.end_page[slot])))
+                    g.reserve(slot, cur + n_new)
+        except CacheError:
+            for g, slot, end in reversed(before):
+                g.shrink(slot, end)
+            raise
+        return starts
 
     def commit(self, slot: int, n_new: int) -> None:
         self._live(slot)

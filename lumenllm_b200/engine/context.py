@@ -148,12 +148,12 @@ class StepLayout:
 
 def pack_step(cache, entries, pad_to: int = 0, table_width: int = 0, want_padding: bool = False,
               pad_lens: Optional[Sequence[int]] = None):
-    """Reserves cache room for the entries and lays the step's metadata out on the host.
+    """Reserves cache room for the entries (for all of them, or on CacheFull for none) and lays the step's metadata out on the host.
     With pad_to > len(entries), padding sequences are appended (of one token each, or of
     pad_lens[i] tokens, which may be none): they start at position 0, their page table is all zeros, so they
     write to the reserved page 0 and are read by nobody (with want_padding the logits at
     their first token are computed too, so that a captured step keeps its shapes)."""
-    starts = [cache.reserve(e.slot, len(e.tokens)) for e in entries]
+    starts = cache.reserve_all([(e.slot, len(e.tokens)) for e in entries])
     B_real = len(entries)
     B = max(B_real, pad_to)
     pads = [1] * (B - B_real) if pad_lens is None else [int(x) for x in pad_lens]
@@ -260,9 +260,9 @@ def build_context(cache, runtime, entries, meta_dev=None, pad_to: int = 0, table
 def tree_context(cache, runtime, entries: Sequence[DraftEntry]):
     """The context of a step that checks drafts. The host sends the tokens, their parents, the slots and the lengths; the
     rest is built on the device (ops.kernels.step_tables). Wanted are the logits at every token. Returns (context,
-    parents on the device); the cache has room for the tokens, nothing is committed."""
+    parents on the device); the cache has room for the tokens (on CacheFull no sequence keeps any), nothing is committed."""
     from ..ops import kernels as K
-    starts = [cache.reserve(e.slot, len(e.tokens)) for e in entries]
+    starts = cache.reserve_all([(e.slot, len(e.tokens)) for e in entries])
     q_lens = [len(e.tokens) for e in entries]
     B, N, longest = len(entries), sum(q_lens), max(q_lens)
     width = max(pages_for(s + q) for s, q in zip(starts, q_lens))
