@@ -286,6 +286,17 @@ class KVCache:
         for g in self.groups:
             g.trim(slot, int(self.lengths[slot]))
 
+    def held_ends(self, slot: int) -> List[int]:
+        """In every group the number of the slot's page that would be its next (see `settle`)."""
+        return [int(g.end_page[slot]) for g in self.groups]
+
+    def settle(self, slot: int, ends: Sequence[int]) -> None:
+        """Gives back the pages that the slot took since it had `ends` (held_ends) and that its tokens do not need: those
+        of drafts that were rejected, or of a step that failed."""
+        last = pages_for(int(self.lengths[slot]))
+        for g, end in zip(self.groups, ends):
+            g.shrink(slot, max(end, last))
+
     def free_tokens(self) -> int:
         return min((g.pool.free_count for g in self.groups), default=self.n_pages) * PAGE
 

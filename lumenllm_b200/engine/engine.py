@@ -251,12 +251,21 @@ class Engine:
         picked at each as generation picks it, and of the drafts those are kept that lie on the path of picked tokens
         from the tree's first token down. Returns the next tokens of each sequence, in the order of the drafts: those kept and
         the one picked behind the last of them, so one at least. The cache then holds the first token and the kept
-        ones; the last returned token is not in it: it is the next step's first.
+        ones, and keeps no page that the step took for more than them; the last returned token is not in it: it is the next step's first.
         `configs`: a SamplingConfig a sequence (without: greedy). `uniforms`: for each sequence as many numbers in [0, 1)
         as its tree is deep, number k for the token picked at depth k (a greedy sequence's row is not read and may be None): with the numbers that single steps would have drawn,
         the tokens are those of single steps (up to the rounding of logits)."""
         drafts = [e if isinstance(e, DraftEntry) else DraftEntry(*e) for e in drafts]
         depths = self._validate_drafts(drafts, configs, uniforms)
+        held = [(e.slot, self.cache.held_ends(e.slot)) for e in drafts]
+        try:
+            return self._verify(drafts, depths, configs, uniforms)
+        finally:
+            # what the tree took beyond the kept tokens, all of it if the step failed
+            for slot, ends in reversed(held):
+                self.cache.settle(slot, ends)
+
+    def _verify(self, drafts, depths, configs, uniforms) -> List[List[int]]:
         try:
             ctx, parents = tree_context(self.cache, self.runtime, drafts)
         except CacheFull as e:

@@ -162,3 +162,36 @@ def test_models_with_state_take_no_drafts():
     s = eng.alloc_slot()
     with pytest.raises(StepError, match="no drafts"):
         eng.verify([DraftEntry(s, [1], [-1])])
+
+
+def test_drafts_that_crowd_the_cache(tiny_models):
+    """Trees as large as the cache's room, mostly wrong: what they took is there again for other sequences, whose pages the
+    page tables on the device follow, and the tokens stay the plain implementation's."""
+    from lumenllm_b200 import DraftEntry, Engine, StepEntry, StepError
+    eng = Engine.from_folder(tiny_models["D"], dtype="float32", max_tokens=512)
+    cfg, w = P.load_model(tiny_models["D"])
+    prompts = seeded_tokens(TINY["D"]["vocab_size"], [50, 64, 10], seed=7)
+    want = [P.generate_greedy(cfg, w, p, 14)[0] for p in prompts]
+    rng = random.Random(3)
+    slots, out = [], []
+    for p, t in zip(prompts, want):
+        slots.append(eng.alloc_slot())
+        eng.step([StepEntry(slots[-1], list(p), [len(p) - 1])])
+        out.append([t[0]])
+    while min(len(o) for o in out) < 12:
+        for b in range(3):
+            room = (eng.cache.free_tokens() // 64 + int(eng.cache.groups[0].end_page[slots[b]])) * 64 - eng.length(slots[b])
+            tokens, parents = grow(rng, [out[b][-1]] + want[b][len(out[b]):], eng.vocab_size, min(room, 200))
+            out[b] += eng.verify([DraftEntry(slots[b], tokens, parents)])[0]
+            eng.cache.check()
+        free = eng.cache.free_tokens()
+        tables = [g.table.copy() for g in eng.cache.groups]
+        with pytest.raises(StepError, match="full"):
+            eng.verify([DraftEntry(s, [1] * 200, [-1] + [0] * 199) for s in slots])
+        assert eng.cache.free_tokens() == free and all((g.table == t).all() for g, t in zip(eng.cache.groups, tables))
+    for b in range(3):
+        n = min(len(out[b]), 14)
+        assert out[b][:n] == want[b][:n]
+        assert eng.cache.groups[0].n_held[slots[b]] == -(-eng.length(slots[b]) // 64)
+        eng.free_slot(slots[b])
+    eng.cache.check()

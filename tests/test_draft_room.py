@@ -73,3 +73,77 @@ def test_a_reservation_that_one_group_refuses_is_none():
             ask()
         assert all(np.array_equal(t, g.table) and n == g.pool.free_count for (t, n), g in zip(before, c.groups))
     assert c.groups[0].pool.free_count == 2 and c.groups[1].pool.free_count == 1
+
+
+class Stopped(RuntimeError):
+    pass
+
+
+def host_only(monkeypatch, eng, kept, fails=None):
+    """The device's part of verify by stand-ins: every sequence keeps kept[slot] tokens of its tree, or `fails` raises Stopped."""
+    import torch
+    from lumenllm_b200.engine import engine as module
+
+    def context(cache, runtime, drafts):
+        cache.reserve_all([(d.slot, len(d.tokens)) for d in drafts])
+        eng.slots_now = [d.slot for d in drafts]
+        return type("C", (), dict(tokens=None, cu_q=None, seq_start=None, block_tables=[None] * len(cache.groups)))(), None
+
+    def stage(name, result):
+        def f(*a, **kw):
+            if fails == name:
+                raise Stopped(name)
+            return result()
+        return f
+
+    accepted = lambda: tuple(torch.tensor(x) for x in
+                             ([kept[s] for s in eng.slots_now], [[0] * 9] * len(eng.slots_now), [[7] * 9] * len(eng.slots_now)))
+    monkeypatch.setattr(module, "tree_context", context)
+    monkeypatch.setattr(module.K, "argmax", lambda logits: None)
+    monkeypatch.setattr(module.K, "tree_accept", stage("accept", accepted))
+    monkeypatch.setattr(module.K, "cache_compact", stage("compact", lambda: None))
+    monkeypatch.setattr(eng, "check_kernels", stage("check", lambda: None), raising=False)
+    eng.model.forward = stage("forward", lambda: None)
+
+
+@pytest.mark.parametrize("window", [0, 40, 100])
+def test_pages_of_rejected_drafts_are_given_back(monkeypatch, window):
+    """After a step of drafts the cache is as after ordinary steps of the kept tokens: a page less than a page's tokens of room."""
+    needs = {0: CacheNeed(1, 16, window), 1: CacheNeed(1, 16)}
+    c, alike = (filled([10, 60, 63], pages=24, needs=needs) for _ in range(2))
+    eng = drafting(c)
+    kept = {0: 1, 1: 5, 2: 1}
+    host_only(monkeypatch, eng, kept)
+    assert eng.verify([star(s, 200) for s in range(3)]) == [[7], [7] * 5, [7]]
+    for s, n in kept.items():
+        alike.reserve(s, n)
+        alike.commit(s, n)
+    assert c.lengths.tolist() == alike.lengths.tolist() == [11, 65, 64, 0, 0]
+    books(c)
+    for g, h in zip(c.groups, alike.groups):
+        assert (g.n_held == h.n_held).all() and (g.end_page == h.end_page).all() and (g.first_page == h.first_page).all()
+        assert ((g.table != 0) == (h.table != 0)).all() and g.pool.free_count == h.pool.free_count
+        assert g._changed >= {0, 1, 2}                   # the rows on the device are out of date
+    # a prompt that fits beside the tokens themselves fits
+    s = c.alloc_slot()
+    c.reserve(s, (24 - 4) * PAGE)
+
+
+def test_room_that_a_slot_had_before_stays_its_own(monkeypatch):
+    c = filled([10], pages=8)
+    c.reserve(0, 3 * PAGE)
+    eng = drafting(c)
+    host_only(monkeypatch, eng, {0: 2})
+    eng.verify([star(0, 250)])
+    assert c.length(0) == 12 and c.groups[0].end_page[0] == 4
+    books(c)
+
+
+@pytest.mark.parametrize("stage", ["forward", "accept", "compact", "check"])
+def test_a_step_of_drafts_that_fails_leaves_the_sequences_as_they_were(monkeypatch, stage):
+    c = filled([10, 60, 64], pages=12, needs={0: CacheNeed(1, 16, 30), 1: CacheNeed(1, 16)})
+    eng, before = drafting(c), books(c)
+    host_only(monkeypatch, eng, {0: 1, 1: 1, 2: 1}, fails=stage)
+    with pytest.raises(Stopped, match=stage):
+        eng.verify([star(s, 150) for s in range(3)])
+    assert same(before, books(c)) and c.lengths.tolist() == [10, 60, 64, 0, 0]
