@@ -28,7 +28,8 @@
 // zeros in the tile before the product reads it, and a row that does see one gets it added at the end.
 //
 // Every wait is bounded, also where warps wait for one another. When one runs out the block raises the error flag, lets the
-// other roles run out, waits for its copies, frees its tensor memory and returns.
+// other roles run out, waits for its copies and products (warps 0 and 1 always do, before the roles meet), frees its tensor memory
+// and returns.
 #pragma once
 #include "tmem_attn.cuh"
 
@@ -398,9 +399,12 @@ attn_tree_tc_kernel(const TreeTc t) {
                 if (++spin > LUMEN_SPIN_LIMIT || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
             }
         }
-        if (lane == 0 && !ok) {
-            *abort_flag = 1;
-            atomicExch(t.err, 1);
+        if (lane == 0) {
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(t.err, 1);
+            }
+            // the last copies have landed before the block ends, also where it is another role that gives up on them
             for (uint32_t i = ck > TT_STAGES ? ck - TT_STAGES : 0; i < ck; ++i) mbar_wait(&k_full[i % TT_STAGES], (i / TT_STAGES) & 1);
             for (uint32_t i = cv > TT_STAGES ? cv - TT_STAGES : 0; i < cv; ++i) mbar_wait(&v_full[i % TT_STAGES], (i / TT_STAGES) & 1);
         }
@@ -496,17 +500,17 @@ attn_tree_tc_kernel(const TreeTc t) {
             }
             if (ok && lane == 0) pt_mbar_arrive(&u_empty[slot]);
         }
-        if (!ok) {
-            // its copies and products in flight end before the tensor memory is given back
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            if (lane == 0) {
+        // its copies and products in flight end before the tensor memory is given back, whichever role gives up
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (lane == 0) {
+            if (!ok) {
                 *abort_flag = 1;
                 atomicExch(t.err, 1);
-                if (cs > 0) mbar_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1);
-                if (cv > 0) mbar_wait(&pv_done[(cv - 1) & 1], ((cv - 1) >> 1) & 1);
             }
-            __syncwarp();
+            if (cs > 0) mbar_wait(&s_full[(cs - 1) & 1], ((cs - 1) >> 1) & 1);
+            if (cv > 0) mbar_wait(&pv_done[(cv - 1) & 1], ((cv - 1) >> 1) & 1);
         }
+        __syncwarp();
     } else {
         const int r = (warp & 3) * 32 + lane;            // this thread's row of a unit
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
