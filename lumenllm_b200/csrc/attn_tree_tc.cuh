@@ -145,7 +145,10 @@ attn_tree_tc_kernel(const TreeTc t) {
     extern __shared__ __align__(1024) unsigned char smem[];
     if (smem_u32(smem) & 1023u) {                       // operand tiles start on 1,024 bytes
         pdl_wait();
-        if (threadIdx.x == 0) atomicExch(t.err, 1);
+        if (threadIdx.x == 0) {
+            t.joins[blockIdx.x] = TreeJoin{0, 0, 0, 0, 0, 0, 1, 0};      // the second kernel finds no pieces
+            atomicExch(t.err, 1);
+        }
         return;
     }
     unsigned char* sQ = smem;

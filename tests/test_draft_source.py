@@ -42,3 +42,12 @@ def test_a_block_waits_for_its_copies_and_products_whichever_role_gives_up(wait)
     assert len(places) == 1
     for cond in conditions_around(text, places[0]):
         assert not re.search(r"\bok\b", cond.split("{")[0]), cond
+
+
+def test_a_block_that_leaves_at_once_leaves_nothing_to_join():
+    """The joining kernel takes its places from every block's record: no way out of the first kernel leaves one unwritten."""
+    text = (CSRC / "attn_tree_tc.cuh").read_text()
+    text = text[text.index("attn_tree_tc_kernel(const TreeTc t) {"):]
+    before = text[:text.index("TreeJoin join = {")]
+    for way_out in [m.start() for m in re.finditer(r"\breturn;", before)]:
+        assert "t.joins[blockIdx.x] =" in before[before.rfind("if (smem_u32", 0, way_out):way_out]
