@@ -98,7 +98,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool tt_warp_wait(uint64_t* bar, uint32_t parity) {
     int ok = 0;
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity);
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();                     // the shuffle alone does not put the other lanes' reads behind what lane 0 has waited for
+    return ok != 0;
 }
 __device__ __forceinline__ bool tt_warp_test(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); }
 // One lane of a whole warp, the same one every time.

@@ -51,3 +51,11 @@ def test_a_block_that_leaves_at_once_leaves_nothing_to_join():
     before = text[:text.index("TreeJoin join = {")]
     for way_out in [m.start() for m in re.finditer(r"\breturn;", before)]:
         assert "t.joins[blockIdx.x] =" in before[before.rfind("if (smem_u32", 0, way_out):way_out]
+
+
+def test_a_warp_whose_first_lane_waits_is_ordered_behind_it():
+    """What one lane has waited for is read by all: a shuffle hands them the answer but orders no memory, a warp barrier does."""
+    text = (CSRC / "attn_tree_tc.cuh").read_text()
+    body = text[text.index("bool tt_warp_wait("):]
+    body = body[:body.index("\n}")]
+    assert body.index("mbar_wait(") < body.index("__syncwarp()") < body.rindex("return")
