@@ -478,12 +478,6 @@ static cudaError_t ta_go(const TreeArgs& a, const int* tok_seq, int max_segs, cu
 #include "attn_tree_mma.cuh"
 #include "attn_tree_tc.cuh"
 
-// Segments that a page table of `width` pages may be cut into.
-static int ta_segs(int width) {
-    const int n = (width + TREE_MIN_SEG - 1) / TREE_MIN_SEG;
-    return n < TREE_MAX_SEGS ? n : TREE_MAX_SEGS;
-}
-
 // Which kernel a call takes whose operands lie on 16 bytes and its output on 32: 1 the tensor cores' (positive: the scale is above 0).
 LUMEN_API int lumen_attn_tree_tc(int is_bf16, int B, int N, int width, int nq, int nkv, int d, int dv, int layout, int v_layout,
                                  int positive) {
@@ -494,7 +488,7 @@ LUMEN_API int lumen_attn_tree_scratch(int tc, int B, int N, int width, int nq, i
     if (B <= 0 || N <= 0 || width < 1 || nkv < 1 || nq < nkv || d < 1 || dv < 1) return 0;
     const int G = nq / nkv;
     const long long n = tc ? tt_floats(tt_blocks(B, N, width, nq, nkv, d, dv), dv)
-                           : ta_segs(width) == 1 ? 0 : (((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2) * nq * (dv + 2);
+                           : tree_max_segs(width) == 1 ? 0 : tree_pairs(B, N, width, G) * nq * (dv + 2);
     return n > 1024LL * 2147483647LL ? -1 : (int)((n + 1023) / 1024);
 }
 
@@ -511,7 +505,7 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
         return LUMEN_ERR_UNSUPPORTED;
     if ((layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || d % 64)) || (v_layout == LUMEN_LAYOUT_SW128 && (!is_bf16 || dv % 64)))
         return LUMEN_ERR_UNSUPPORTED;
-    const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = ta_segs(width);
+    const int G = nq / nkv, es = is_bf16 ? 2 : 4, max_segs = tree_max_segs(width);
     if ((long long)N * G > (1 << 30) || ((long long)N * G / TA_ROWS + B) * nkv > 2147483647LL || (long long)(dv + 3) / 4 * nq > 128LL * 65535) return LUMEN_ERR_UNSUPPORTED;
     const int need = lumen_attn_tree_scratch(tc, B, N, width, nq, nkv, d, dv);
     if (need < 0) return LUMEN_ERR_UNSUPPORTED;
@@ -521,12 +515,12 @@ LUMEN_API int lumen_attn_tree(const void* q, const void* kcache, const void* vca
     const int vec = (((uintptr_t)kcache & 15) == 0 && d * es % 16 == 0 ? 1 : 0) | (((uintptr_t)vcache & 15) == 0 && dv * es % 16 == 0 ? 2 : 0) |
                     (((uintptr_t)q & 15) == 0 && d * es % 16 == 0 ? 4 : 0);
     // the maxima and sums first: the rows behind them lie on 16 bytes where dv is a multiple of 4
-    const long long pairs = ((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2;
+    const long long pairs = tree_pairs(B, N, width, G);
     TreeArgs a = {q, kcache, vcache, block_table, cu_q, seq_start, tok_pos, (const unsigned long long*)mask, out,
                         scratch ? scratch + pairs * nq * 2 : nullptr, (float2*)scratch, sink, bt_stride, width, W, B, N, n_pages, nq, nkv,
                         d, dv, window, layout, v_layout, vec, TREE_MIN_SEG, TREE_SEG_ROWS, scale, softcap};
     const bool mma = !tc && tm_takes(a, is_bf16);
-    if (mma) { a.seg_min = 4; a.seg_rows = 16; }
+    if (mma) { a.seg_min = TREE_MMA_MIN_SEG; a.seg_rows = TREE_MMA_SEG_ROWS; }
     cudaError_t e;
 #define TA_GO(T) (dv <= 128 ? ta_go<T, 1>(a, tok_seq, max_segs, stream) : dv <= 256 ? ta_go<T, 2>(a, tok_seq, max_segs, stream) \
                                                                                    : ta_go<T, 4>(a, tok_seq, max_segs, stream))

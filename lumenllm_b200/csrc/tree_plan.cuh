@@ -10,6 +10,8 @@
 #define TREE_MAX_SEGS 64          // a sequence is never cut into more segments than this
 #define TREE_MIN_SEG 2            // pages of the shortest segment
 #define TREE_SEG_ROWS 32          // rows that have a page of a segment to themselves, at most
+#define TREE_MMA_MIN_SEG 4        // both for the mma.sync kernel
+#define TREE_MMA_SEG_ROWS 16
 
 struct TreeSeq {
     int n0, q;        // its first token of the step, its nodes
@@ -27,7 +29,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const int* cu_q, const int* seq_star
 }
 
 // Pages [pg_lo, pg_lo + np) are those that some node of the sequence may see.
-__device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg_lo, int& np) {
+__host__ __device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg_lo, int& np) {
     // no node stands before the cached tokens' end
     const int lo = window > 0 ? min(max(0, s.start - window + 1), s.end - 1) : 0;
     pg_lo = lo / LUMEN_PAGE;
@@ -40,10 +42,10 @@ __device__ __forceinline__ void tree_pages(const TreeSeq& s, int window, int& pg
 // width.
 struct TreePlan {
     int pg_lo, np, nseg, per, rem;
-    __device__ __forceinline__ int first(int seg) const { return pg_lo + seg * per + min(seg, rem); }
-    __device__ __forceinline__ int count(int seg) const { return per + (seg < rem ? 1 : 0); }
+    __host__ __device__ __forceinline__ int first(int seg) const { return pg_lo + seg * per + min(seg, rem); }
+    __host__ __device__ __forceinline__ int count(int seg) const { return per + (seg < rem ? 1 : 0); }
 };
-__device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int G, int seg_min, int seg_rows) {
+__host__ __device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int G, int seg_min, int seg_rows) {
     TreePlan p;
     tree_pages(s, window, p.pg_lo, p.np);
     const long long rows = (long long)s.q * G;
@@ -56,8 +58,13 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeSeq& s, int window, int 
 // Partial results of sequence b lie from this (token, segment) pair on, node i's segments at i * nseg: q * nseg is at most
 // q + TREE_SEG_ROWS width / G whatever the lengths are (seg_min TREE_MIN_SEG or more, seg_rows TREE_SEG_ROWS or less).
 __host__ __device__ __forceinline__ long long tree_part_room(int width, int G) { return ((long long)TREE_SEG_ROWS * width + G - 1) / G; }
-__device__ __forceinline__ long long tree_part_base(int b, int n0, int width, int G) {
+__host__ __device__ __forceinline__ long long tree_part_base(int b, int n0, int width, int G) {
     return (long long)b * tree_part_room(width, G) + n0;
+}
+// Segments that the pages of a table of `width` pages may be cut into, and (token, segment) pairs of all sequences.
+__host__ __device__ __forceinline__ int tree_max_segs(int width) { return min((width + TREE_MIN_SEG - 1) / TREE_MIN_SEG, TREE_MAX_SEGS); }
+__host__ __device__ __forceinline__ long long tree_pairs(int B, int N, int width, int G) {
+    return ((long long)B * tree_part_room(width, G) + N + 1) / 2 * 2;
 }
 
 // Unit u of a step whose sequences have ceil(q G / rows) tiles of rows each, in the order of the sequences: the sequence
